@@ -501,6 +501,57 @@ int mta_rows_copy(int count, const void *const *x, const int64_t *x_strides, voi
 int mta_probe_head_weight(const void *w, int64_t H, int w_dtype, int32_t *out, void *stream);
 int mta_probe_conv_kernel(const void *w, int64_t C, int R, int S, int w_dtype, int32_t *out, void *stream);
 
+/* ---- single-token attention over a paged cache --------------------------------------------------------------------
+ * The serving form of the two attention modules; the reference has none (its modules compute whole sequences:
+ * mta_attention_triton.py:60-92, conv_attention_triton.py:362-452).
+ *
+ * A cache of `slots` sequences.  Keys and values lie in pages: k, v are (n_pages, kv_heads, page, head_dim), page a power of
+ * two from 16 to 1024; table is int32 (slots, max_pages), entry i of a slot names the page of its positions i * page ..
+ * (entries behind the last token may hold anything).  q is (slots, heads, query_rows, head_dim): the newest queries, the one of
+ * position i in row i % query_rows.  state is int32 (2, slots): the tokens that a slot held, and those that it got in the last
+ * extension; a slot that got none sits the step out.  Query head h reads key head h / (heads / kv_heads).  table and state are
+ * read on the device when the work runs: a captured graph follows them.
+ *
+ * Kernels check what they read there.  A slot whose state is no state of this cache (more tokens than `longest` of the call or
+ * than its row of the table has room for, a negative number), or one of whose pages is none of 0 .. n_pages - 1, gets NaN for
+ * a result, and nothing is read or written through such an entry. */
+typedef struct mta_cache {
+    void *k, *v, *q;
+    const int32_t *table, *state;
+    int64_t n_pages;
+    int32_t slots, max_pages, page, heads, kv_heads, head_dim, query_rows, dtype;
+} mta_cache;
+
+/* New tokens into the cache: token i of slot b, i < state[1][b], goes to position state[0][b] + i; the newest query_rows queries
+ * of a slot go to the ring.  xq is (slots, heads, tokens, head_dim), xk and xv (slots, kv_heads, tokens, head_dim), elements of a
+ * row contiguous; strides: (slot, head, token) in elements of xq, of xk, of xv, nine numbers, multiples of 16 bytes. */
+int mta_cache_append(const mta_cache *cache, const void *xq, const void *xk, const void *xv, const int64_t *strides, int64_t tokens, void *stream);
+
+/* page pairs[2 i + 1] = page pairs[2 i], i < n, in both pools of n_pages pages of page_bytes bytes; pairs lies in host memory and is
+ * read before the call returns.  A page may be the source of several pairs; the caller sees to it that no page is the target of two,
+ * or target of one and source of another (the order of the copies is not defined). */
+int mta_cache_copy_pages(void *k, void *v, int64_t n_pages, int64_t page_bytes, const int32_t *pairs, int64_t n, void *stream);
+
+/* Fused conv-attention (mta_conv_attn_fwd, causal) of the newest token p of every slot that got tokens:
+ *   o[b,h] = softmax_k( scale * sum_{r,t} w[h,r,t] raw_{p-R+1+r}[k+t-(S-1)/2] ) V,   raw_i[k] = q_i . k_k, or 0 where row i does not see
+ * key k: it sees max(0, i - window + 1) .. i (window = 0: from key 0 on).  o is (slots, heads, head_dim), zeros for slots that sit out.
+ * query_rows >= R.  Everything between the inputs and o is held in fp32.  longest: no slot holds more tokens (state counted in full);
+ * it sizes the grid and the workspace.  The workspace call returns bytes, or an error code. */
+int64_t mta_conv_attn_decode_workspace(const mta_cache *cache, int64_t longest, int R, int S, int window);
+int mta_conv_attn_decode(const mta_cache *cache, const void *w, void *o, void *workspace, int64_t workspace_bytes, int64_t longest, int R, int S,
+                         int window, float scale, int w_dtype, void *stream);
+
+/* Multi-Token Attention (mta_attention_triton.py:60-92, causal) of the newest token of every slot that got tokens: with the
+ * rows j = p - R2 + 1 .. p,  p_j = softmax( w_pre mix of conv_w(scale * raw) ),  o = ( w_post mix of conv_w2(p) at row p ) V;
+ * what a row does not see counts as 0 ahead of either conv.  w is (heads, R, S), w2 (heads, R2, S2) or NULL with R2 = S2 = 1 (the
+ * identity), w_pre and w_post (heads, heads) or NULL (the identity), all of dtype w_dtype; pre_group, post_group as group_size of
+ * mta_headmix_fwd.  query_rows >= R + R2 - 1.  Everything else as mta_conv_attn_decode; the workspace (8-byte aligned) serves any
+ * choice of NULL weights. */
+int64_t mta_decode_workspace(const mta_cache *cache, int64_t longest, int R, int S, int R2, int S2, int pre_group, int post_group, int window);
+int mta_decode(const mta_cache *cache, const void *w, const void *w_pre, const void *w2, const void *w_post, void *o, void *workspace,
+               int64_t workspace_bytes, int64_t longest, int R, int S, int R2, int S2, int pre_group, int post_group, int window, float scale,
+               int w_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,6 +27,12 @@ class Partials(_c.Structure):
                 ("mask", _c.c_int32), ("dtype", _c.c_int32), ("scale", _f32)]
 
 
+class Cache(_c.Structure):
+    """mta_cache of include/mta_hip.h"""
+    _fields_ = [("k", _vp), ("v", _vp), ("q", _vp), ("table", _vp), ("state", _vp), ("n_pages", _i64), ("slots", _c.c_int32), ("max_pages", _c.c_int32),
+                ("page", _c.c_int32), ("heads", _c.c_int32), ("kv_heads", _c.c_int32), ("head_dim", _c.c_int32), ("query_rows", _c.c_int32), ("dtype", _c.c_int32)]
+
+
 # name -> (restype, argtypes); one entry per declaration in include/mta_hip.h
 SIGNATURES = {
     "mta_abi_version": (_int, []),
@@ -97,6 +103,12 @@ SIGNATURES = {
     "mta_causal_ptx_f32": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _vp]),
     "mta_probe_head_weight": (_int, [_vp, _i64, _int, _vp, _vp]),
     "mta_probe_conv_kernel": (_int, [_vp, _i64, _int, _int, _int, _vp, _vp]),
+    "mta_cache_append": (_int, [_vp] * 5 + [_i64, _vp]),
+    "mta_cache_copy_pages": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "mta_conv_attn_decode_workspace": (_i64, [_vp, _i64, _int, _int, _int]),
+    "mta_conv_attn_decode": (_int, [_vp] * 4 + [_i64, _i64, _int, _int, _int, _f32, _int, _vp]),
+    "mta_decode_workspace": (_i64, [_vp, _i64] + [_int] * 7),
+    "mta_decode": (_int, [_vp] * 7 + [_i64, _i64] + [_int] * 7 + [_f32, _int, _vp]),
     "mta_conv_attn_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _f32, _int, _int, _vp]),
 }
 

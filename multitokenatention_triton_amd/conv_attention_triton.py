@@ -63,3 +63,14 @@ class TritonConvAttention(nn.Module):
         # (nothing to differentiate: no row statistic is written)
         assert weight.size(0) == Q.size(1)
         return _lib.host().conv_attn(Q, K, V, weight, causal, softmax_scale), None
+
+    @property
+    def decode_query_rows(self) -> int:
+        """Queries per sequence that ``decode`` needs a cache to keep."""
+        return self.kernel_size[0]
+
+    def decode(self, cache, softmax_scale=None, window=0):
+        """The row of the newest token of every slot of a ``PagedCache`` that got tokens in its last ``extend``: (slots, H, 1, D),
+        zeros for the other slots.  Causal; ``window``: a row sees that many keys at most, itself included (0: all).  What
+        forward() rounds to the dtype between its stages stays in fp32 here.  No gradients."""
+        return _lib.host().conv_attn_decode(cache.k, cache.v, cache.q, cache.table, cache.state, cache.longest, self.weight.detach(), softmax_scale, window)

@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/anomaly_mode.h>
 
 #include "ops.hpp"
+#include "decode.hpp"
 
 namespace py = pybind11;
 
@@ -972,4 +973,8 @@ PYBIND11_MODULE(_host, m)
     m.def("conv2d_apply", &conv2d_apply);
     m.def("headmix_apply", &headmix_apply);
     m.def("conv_attn", &conv_attn);
+    m.def("conv_attn_decode", &conv_attn_decode);
+    m.def("mta_decode", &mta_decode_step);
+    m.def("cache_append", &cache_append);
+    m.def("cache_copy_pages", &cache_copy_pages);
 }

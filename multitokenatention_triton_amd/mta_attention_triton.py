@@ -403,6 +403,30 @@ class MTAAttentionTriton(nn.Module):
         self._mark("end")
         return output.transpose(1, 2)
 
+    # ------------------------------------------------------------------ one token at a time
+    @property
+    def decode_query_rows(self) -> int:
+        """Queries per sequence that ``decode`` needs a cache to keep: both convs reach back over query rows."""
+        return self.mta_conv_triton.weight.size(1) + self.mta_conv_after_sm_triton.weight.size(1) - 1
+
+    def decode(self, cache, window: int = 0):
+        """The row of the newest token of every slot of a ``PagedCache`` that got tokens in its last ``extend``: (slots, 1, H, D),
+        zeros for the other slots.  ``window``: a row sees that many keys at most, itself included (0: all), as a sliding-window
+        mask does in forward().  What forward() rounds to the dtype between its stages stays in fp32 here.  No gradients,
+        no dropout.  A known weight structure is used as in inference."""
+        if not self.causal:
+            raise ValueError("decode is causal by construction: a module with causal=False needs the whole sequence")
+        if self.training and self.dropout > 0:
+            raise RuntimeError("decode has no dropout: call eval() first")
+        st = self._current_structure()
+        conv, pre, post_conv, post = (w.detach() for w in self._weights())
+        args = (cache.k, cache.v, cache.q, cache.table, cache.state, cache.longest)
+        host = _lib.host()
+        if st.pre_head_identity and st.post_conv_identity and st.post_head_identity:   # (conv-attention: one pass)
+            return host.conv_attn_decode(*args, conv, None, window).transpose(1, 2)
+        return host.mta_decode(*args, conv, None if st.pre_head_identity else pre, None if st.post_conv_identity else post_conv,
+                               None if st.post_head_identity else post, st.pre_head_group or 0, st.post_head_group or 0, window)
+
     # ------------------------------------------------------------------ weight structure
     def _current_structure(self) -> "WeightStructure":
         if self.weight_structure == "dense":
