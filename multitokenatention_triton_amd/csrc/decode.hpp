@@ -94,6 +94,7 @@ __device__ __forceinline__ float wave_sum(float v) { return wave_reduce(v, [](fl
 template <int STEP> __device__ __forceinline__ float lanes_sum(float v)
 {
     auto add = [](float a, float b) { return a + b; };
+    if constexpr (STEP <= 4) v = v + dpp<0x124>(v);
     if constexpr (STEP <= 8) v = v + dpp<0x128>(v);
     if constexpr (STEP <= 16) v = across16(v, add);
     if constexpr (STEP <= 32) v = across32(v, add);
@@ -135,8 +136,11 @@ template <typename T> __device__ __forceinline__ wide<T> widen(const u32x4 &x)
 // ---- sizes that kernels and host agree on ----
 __host__ __device__ __forceinline__ int halo_left(int S) { return (((S - 1) / 2) + 15) & ~15; }
 __host__ __device__ __forceinline__ int halo_right(int S) { return (S - 1 - (S - 1) / 2 + 15) & ~15; }
-// columns of a row of raw scores: the halos, a step's keys, and 4 more, which spreads the four row groups of an accumulator over the banks
-__host__ __device__ __forceinline__ int raw_stride(int S, int nt) { return halo_left(S) + halo_right(S) + 64 * nt + 4; }
+// ahead of the first column, so that the taps of a key that is a multiple of 4 begin on 16 bytes
+__host__ __device__ __forceinline__ int raw_shift(int S) { return ((S - 1) / 2 - halo_left(S)) & 3; }
+// columns of a row of raw scores: shift, halos, a step's keys, and what a window of whole vectors reads behind them; 12 more than a multiple
+// of 16, which spreads the four row groups of an accumulator over the banks
+__host__ __device__ __forceinline__ int raw_stride(int S, int nt) { return halo_left(S) + halo_right(S) + 64 * nt + 12; }
 __host__ __device__ __forceinline__ int q_stride(int row_bytes) { return row_bytes + 32; }   // (conflict-free fragment reads)
 __host__ __device__ __forceinline__ int up16(int x) { return (x + 15) & ~15; }
 
@@ -209,29 +213,53 @@ template <typename T, int D, int NT> struct raw_scores {
 #pragma unroll
         for (int t = 0; t < NT; ++t) bad |= load(kreg[t], first_of(kb, t)) ? 0 : 1 << t;
     }
-    // the scores of a tile: to column `col` of a buffer and, col2 >= 0, to column col2 of another
-    __device__ __forceinline__ void score(const u32x4 (&kr)[NC], int key0, bool is_bad, float *buf, int col, float *buf2, int col2) const
+    // The scores of N tiles from key0 on, 16 query rows after 16: to column `col` of a buffer and, where they are the first columns of the next
+    // step, of that one's.
+    template <int N> __device__ __forceinline__ void score(const u32x4 (&kr)[N][NC], int key0, int is_bad, float *buf, int col, float *next) const
     {
-        const int key = key0 + (lane & 15);
+        const int group = lane >> 4, at = lane & 15;
+        // (all rows see all of these keys: nothing to replace)
+        const bool plain = is_bad == 0 && a.window == 0 && key0 >= 0 && key0 + 16 * N - 1 <= n - a.W;
         for (int m0 = 0; m0 < rows; m0 += 16) {
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            const unsigned char *qrow = qs + (m0 + (lane & 15)) * q_stride(ROW) + (lane >> 4) * 16;
+            f32x4 acc[N];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) mma_rows<T>(acc, *reinterpret_cast<const u32x4 *>(qrow + 64 * c), kr[c]);
-            const int r0 = m0 + 4 * (lane >> 4);
+            for (int t = 0; t < N; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const unsigned char *qrow = qs + (m0 + at) * q_stride(ROW) + group * 16;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const u32x4 qv = *reinterpret_cast<const u32x4 *>(qrow + 64 * c);
+#pragma unroll
+                for (int t = 0; t < N; ++t) mma_rows<T>(acc[t], qv, kr[t][c]);
+            }
+            const int r0 = m0 + 4 * group;
+            if (!plain) {
+                const int4 p = *reinterpret_cast<const int4 *>(pos + r0);
+                const int ps[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int t = 0; t < N; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        // (what a row does not see is replaced, not multiplied: garbage behind the last key stays out)
+                        const int key = key0 + 16 * t + at;
+                        const bool seen = key >= 0 && key <= ps[v] && (a.window == 0 || key > ps[v] - a.window);
+                        acc[t][v] = !seen ? 0.0f : is_bad >> t & 1 ? __builtin_nanf("") : acc[t][v];
+                    }
+            }
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 if (r0 + v >= rows) break;
-                const int p = pos[r0 + v];
-                // (what a row does not see is replaced, not multiplied: garbage behind the last key stays out)
-                const bool seen = key >= 0 && key <= p && (a.window == 0 || key > p - a.window);
-                const float x = !seen ? 0.0f : is_bad ? __builtin_nanf("") : acc[v];
-                buf[(r0 + v) * stride + col + (lane & 15)] = x;
-                if (col2 >= 0) buf2[(r0 + v) * stride + col2 + (lane & 15)] = x;
+                float *const to = buf + (r0 + v) * stride + col + at;
+#pragma unroll
+                for (int t = 0; t < N; ++t) to[16 * t] = acc[t][v];
+                if (next) {
+#pragma unroll
+                    for (int t = 0; t < N; ++t)
+                        if (col + 16 * t >= CH) next[(r0 + v) * stride + col + 16 * t - CH + at] = acc[t][v];
+                }
             }
         }
     }
-    __device__ __forceinline__ float *buffer(int step) const { return raw + (step % 3) * rows * stride; }
+    __device__ __forceinline__ float *buffer(int step) const { return raw + raw_shift(a.S) + (step % 3) * rows * stride; }
     // Query rows, their positions and the conv weights into LDS: rows g * W + i, position p - W + 1 + i of query head h0 + g.
     __device__ __forceinline__ void stage(unsigned char *smem, const raw_layout &l, int b, int h0) const
     {
@@ -255,21 +283,83 @@ template <typename T, int D, int NT> struct raw_scores {
     __device__ __forceinline__ void halo(int kb) const
     {
         if (wave * 16 >= hl + hr) return;
-        u32x4 kr[NC];
+        u32x4 kr[1][NC];
         const int key0 = kb - hl + wave * 16;
-        const bool ok = load(kr, key0);
-        score(kr, key0, !ok, buffer(0), wave * 16, nullptr, -1);
+        const bool ok = load(kr[0], key0);
+        score<1>(kr, key0, !ok, buffer(0), wave * 16, nullptr);
     }
     // this step's scores, from the keys that load_step() brought
     __device__ __forceinline__ void score_step(int kb, int step) const
     {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int col = hl + hr + (wave * NT + t) * 16;
-            score(kreg[t], first_of(kb, t), bad >> t & 1, buffer(step), col, buffer(step + 1), col >= CH ? col - CH : -1);
-        }
+        const int col = hl + hr + wave * NT * 16;
+        score<NT>(kreg, first_of(kb, 0), bad, buffer(step), col, col + NT * 16 > CH ? buffer(step + 1) : nullptr);
+    }
+    // where the taps of the step's key `local` begin in row `row` of a buffer
+    __device__ __forceinline__ const float *window(int step, int row, int local) const
+    {
+        return buffer(step) + row * stride + local + hl - (a.S - 1) / 2;
     }
 };
+
+// ---- the conv: a lane forms four neighbouring keys, whose taps it reads as whole vectors ----
+// c[u] += sum over t < S of w[t] x[t + u]; x and w begin on 16 bytes.  Taps behind the last one are left out, not multiplied by 0 (a score may
+// be infinite).  N: their number, 0: only known at run time.
+template <int N> __device__ __forceinline__ void taps4(float (&c)[4], const float *x, const float *w, int S)
+{
+    if constexpr (N > 0) {
+        constexpr int V = (N + 6) / 4;
+        float xs[4 * V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) *reinterpret_cast<f32x4 *>(xs + 4 * i) = *reinterpret_cast<const f32x4 *>(x + 4 * i);
+        float ws[4 * ((N + 3) / 4)];
+#pragma unroll
+        for (int i = 0; i < (N + 3) / 4; ++i) *reinterpret_cast<f32x4 *>(ws + 4 * i) = *reinterpret_cast<const f32x4 *>(w + 4 * i);
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) c[u] = fmaf(ws[t], xs[t + u], c[u]);
+    } else {
+        f32x4 lo = *reinterpret_cast<const f32x4 *>(x);
+        for (int t0 = 0; t0 < S; t0 += 4) {
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(x + t0 + 4), wv = *reinterpret_cast<const f32x4 *>(w + t0);
+            const float xs[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (t0 + t < S) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) c[u] = fmaf(wv[t], xs[t + u], c[u]);
+                }
+            lo = hi;
+        }
+    }
+}
+template <int N> struct count_of { static constexpr int value = N; };
+// f(count_of<S>) for the sizes with unrolled code, f(count_of<0>) for the others
+template <typename F> __device__ __forceinline__ void with_taps(int S, F f)
+{
+    switch (S) {
+    case 3: f(count_of<3>()); break;
+    case 5: f(count_of<5>()); break;
+    case 7: f(count_of<7>()); break;
+    case 9: f(count_of<9>()); break;
+    case 11: f(count_of<11>()); break;
+    case 15: f(count_of<15>()); break;
+    default: f(count_of<0>()); break;
+    }
+}
+// Four values per lane, for the keys 4 * (lane % (4 NT)) .. + 3, partial over the lanes of equal lane % (4 NT): the whole sum of key
+// 4 * (lane % (4 NT)) + lane / 16 in every lane.  Halves and rows change places as they are added, so a value is moved once and not four times.
+template <int NT> __device__ __forceinline__ float deal4(float (&c)[4])
+{
+    swap32(c[0], c[2]);
+    swap32(c[1], c[3]);
+    uint32_t p = __float_as_uint(c[0] + c[2]), q = __float_as_uint(c[1] + c[3]);   // lower half: keys 0 and 1, upper half: 2 and 3
+    swap16(p, q);
+    float v = __uint_as_float(p) + __uint_as_float(q);
+    if constexpr (NT <= 2) v += dpp<0x128>(v);
+    if constexpr (NT == 1) v += dpp<0x124>(v);
+    return v;
+}
 
 // A wavefront's 16 * NT rows of V times the probabilities of GW heads: a row is read by ROW / 16 lanes.
 template <typename T, int D, int NT, int GW> struct value_rows {

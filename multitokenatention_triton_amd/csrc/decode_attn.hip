@@ -27,11 +27,12 @@ __global__ __launch_bounds__(256) void conv_attn_decode_kernel(const decode_args
     if (beg >= s.n) return;
     const int end = beg + a.split_len < s.n ? beg + a.split_len : s.n;
 
-    constexpr int CH = 64 * NT, SUBS = 4 / NT;   // (a key's taps are dealt over SUBS lanes)
+    constexpr int CH = 64 * NT, QUADS = 4 * NT, SUBS = 64 / QUADS;   // (four keys per lane, a key's rows of taps dealt over SUBS lanes)
     const int rows = GW * a.R, left = (a.S - 1) / 2, reach = end + a.S - 1 - left;
     const raw_layout l = raw_layout_of(rows, a.R, a.S, GW, D, (int)sizeof(T), NT, true);
     raw_scores<T, D, NT> sc(a, smem, l, rows, b, h0 / a.share, s.n, reach < s.n ? reach : s.n);
-    const int lane = sc.lane, wave = sc.wave, sub = lane / (16 * NT), mine = lane % (16 * NT);
+    const int lane = sc.lane, wave = sc.wave, quad = lane % QUADS, sub = lane / QUADS, mine = 4 * quad + lane / 16;
+    const bool owner = lane % 16 < QUADS;   // (with NT < 4 several lanes come to hold the same key)
     const float *const weights = reinterpret_cast<const float *>(smem + l.weights);
     float *const probs = reinterpret_cast<float *>(smem + l.probs) + wave * GW * 16 * NT;
     const int sp = (a.S + 3) & ~3;
@@ -57,26 +58,14 @@ __global__ __launch_bounds__(256) void conv_attn_decode_kernel(const decode_args
         __syncthreads();
         const int key = first + mine;
         const bool seen = key >= s.lo && key < end;
-        const float *const x0 = sc.buffer(step) + wave * 16 * NT + mine + sc.hl - left;
 #pragma unroll
         for (int g = 0; g < GW; ++g) {
-            float c = 0.0f;
-            for (int r = 0; r < a.R; ++r) {
-                const float *x = x0 + (g * a.R + r) * sc.stride, *w = weights + (g * a.R + r) * sp;
-                if constexpr (SUBS == 1) {
-                    int t = 0;
-                    for (; t + 4 <= a.S; t += 4) {
-                        const f32x4 w4 = *reinterpret_cast<const f32x4 *>(w + t);
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) c = fmaf(w4[u], x[t + u], c);
-                    }
-                    for (; t < a.S; ++t) c = fmaf(w[t], x[t], c);
-                } else {
-                    for (int t = sub; t < a.S; t += SUBS) c = fmaf(w[t], x[t], c);
-                }
-            }
-            if constexpr (SUBS >= 2) c = across32(c, [](float p, float q) { return p + q; });
-            if constexpr (SUBS == 4) c = across16(c, [](float p, float q) { return p + q; });
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            with_taps(a.S, [&](auto count) {
+                for (int r = sub; r < a.R; r += SUBS)
+                    taps4<decltype(count)::value>(part, sc.window(step, g * a.R + r, wave * 16 * NT + 4 * quad), weights + (g * a.R + r) * sp, a.S);
+            });
+            const float c = deal4<NT>(part);
             const float e = seen ? c * scale2 : -INFINITY;
             const float top = fmaxf(m[g], wave_max(e));
             if (top > m[g]) {   // (wavefront-uniform)
@@ -88,7 +77,7 @@ __global__ __launch_bounds__(256) void conv_attn_decode_kernel(const decode_args
             }
             // (no score but -inf so far: a reference of 0, so that such keys count 0 and not NaN)
             const float p = seen ? __builtin_amdgcn_exp2f(e - (m[g] == -INFINITY ? 0.0f : m[g])) : 0.0f;
-            if (sub == 0) {
+            if (owner) {
                 sum[g] += p;
                 probs[g * 16 * NT + mine] = p;
             }
@@ -134,13 +123,13 @@ __global__ __launch_bounds__(256) void conv_attn_decode_kernel(const decode_args
     }
 }
 
-// The splits of one (slot, head), brought to one reference and added up in their order.
+// The splits of one (slot, head), brought to one reference and added up, always in the same order.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a)
 {
     constexpr int PARTS = 256 / D;
-    __shared__ float so[PARTS][D], st[PARTS];
-    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D;
+    __shared__ float so[PARTS][D], factor[64];
+    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D, lane = threadIdx.x & 63;
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
     const slot_step s = step_of(a, b, 0);
     if (s.n <= 0) {
@@ -149,22 +138,30 @@ __global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a
     }
     const int splits = (s.n - s.base + a.split_len - 1) / a.split_len;
     const int64_t at = ((int64_t)b * a.heads + h) * a.n_splits;
-    const float *o = a.ws + at * D, *ml = a.ws + stats_offset(a.slots, a.heads, a.n_splits, D) + 2 * at;
+    const float *o = a.ws + at * D;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + stats_offset(a.slots, a.heads, a.n_splits, D)) + at;
     float top = -INFINITY;
-    for (int i = 0; i < splits; ++i) top = fmaxf(top, ml[2 * i]);
+    for (int i = lane; i < splits; i += 64) top = fmaxf(top, ml[i].x);
+    top = wave_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, total = 0.0f;
-    for (int i = part; i < splits; i += PARTS) {
-        const float f = exp2f(ml[2 * i] - ref);
-        sum = fmaf(f, o[(int64_t)i * D + d], sum);
-        total = fmaf(f, ml[2 * i + 1], total);
+    for (int i0 = 0; i0 < splits; i0 += 64) {   // (factors of 64 splits at a time; all wavefronts form the same ones)
+        const float2 x = i0 + lane < splits ? ml[i0 + lane] : make_float2(-INFINITY, 0.0f);
+        const float f = __builtin_amdgcn_exp2f(x.x - ref);
+        total += f * x.y;
+        __syncthreads();
+        if (threadIdx.x < 64) factor[lane] = f;
+        __syncthreads();
+        const int most = splits - i0 < 64 ? splits - i0 : 64;
+#pragma unroll 8
+        for (int i = part; i < most; i += PARTS) sum = fmaf(factor[i], o[(int64_t)(i0 + i) * D + d], sum);
     }
+    total = wave_sum(total);
     so[part][d] = sum;
-    if (d == 0) st[part] = total;
     __syncthreads();
     if (part != 0) return;
 #pragma unroll
-    for (int i = 1; i < PARTS; ++i) sum += so[i][d], total += st[i];
+    for (int i = 1; i < PARTS; ++i) sum += so[i][d];
     out[d] = from_float<T>(sum / total);
 }
 
@@ -238,7 +235,7 @@ extern "C" int mta_conv_attn_decode(const mta_cache *c, const void *w, void *o, 
     if (const int e = check_args(c, longest, R, S, window)) return e;
     if (!w || !o) return MTA_ERR_NULL;
     if (dtype_size(w_dtype) == 0) return MTA_ERR_DTYPE;
-    if (!aligned_to(w, dtype_size(w_dtype)) || !aligned_to(o, dtype_size(c->dtype)) || !aligned_to(workspace, 4)) return MTA_ERR_ALIGN;
+    if (!aligned_to(w, dtype_size(w_dtype)) || !aligned_to(o, dtype_size(c->dtype)) || !aligned_to(workspace, 8)) return MTA_ERR_ALIGN;
     plan p;
     if (const int e = plan_of(c, longest, R, S, window, p)) return e;
     const int64_t need = mta_conv_attn_decode_workspace(c, longest, R, S, window);

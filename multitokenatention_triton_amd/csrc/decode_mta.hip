@@ -33,7 +33,9 @@ __device__ __forceinline__ int row_pos(const mta_args &a, int n, int j) { return
 __device__ __forceinline__ bool sees(const mta_args &a, int pos, int key) { return key >= 0 && key <= pos && (a.d.window == 0 || key > pos - a.d.window); }
 
 // ---- scores: K once ----
-template <typename T, int D, int NT, int JB>
+// R2 = 1: as in conv-attention a key's rows of taps are dealt over the lanes that share it.  Else the output rows are, JB to a lane: a window of
+// raw scores is read once for all of them.
+template <typename T, int D, int NT, int JB, bool ONE>
 __global__ __launch_bounds__(256) void decode_scores_kernel(const mta_args m)
 {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -45,11 +47,11 @@ __global__ __launch_bounds__(256) void decode_scores_kernel(const mta_args m)
     if (beg >= s.n) return;
     const int end = beg + a.split_len < s.n ? beg + a.split_len : s.n;
 
-    constexpr int CH = 64 * NT, SUBS = 4 / NT;
+    constexpr int CH = 64 * NT, QUADS = 4 * NT, SUBS = 64 / QUADS;
     const int rows = a.gw * a.W, left = (a.S - 1) / 2, reach = end + a.S - 1 - left;
     const raw_layout l = raw_layout_of(rows, a.R, a.S, a.gw, D, (int)sizeof(T), NT, false);
     raw_scores<T, D, NT> sc(a, smem, l, rows, b, h0 / a.share, s.n, reach < s.n ? reach : s.n);
-    const int lane = sc.lane, wave = sc.wave, sub = lane / (16 * NT), mine = lane % (16 * NT);
+    const int lane = sc.lane, wave = sc.wave, quad = lane % QUADS, sub = lane / QUADS;
     const float *const weights = reinterpret_cast<const float *>(smem + l.weights);
     const int sp = (a.S + 3) & ~3;
 
@@ -62,33 +64,39 @@ __global__ __launch_bounds__(256) void decode_scores_kernel(const mta_args m)
         sc.score_step(kb, step);
         if (kb + CH < end) sc.load_step(kb + CH);
         __syncthreads();
-        const int key = kb + wave * 16 * NT + mine;
-        const float *const x0 = sc.buffer(step) + wave * 16 * NT + mine + sc.hl - left;
-        for (int g = 0; g < a.gw; ++g)
-            for (int j0 = 0; j0 < m.R2; j0 += JB) {   // (a raw score serves JB rows)
-                float c[JB];
+        const int local = wave * 16 * NT + 4 * quad, key = kb + local;
+        float *const out = m.s1 + ((int64_t)b * a.heads + h0) * m.R2 * m.span + (key - s.base);
+        for (int g = 0; g < a.gw; ++g) {
+            const float *const w = weights + g * a.R * sp;
+            if constexpr (ONE) {
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                with_taps(a.S, [&](auto count) {
+                    for (int r = sub; r < a.R; r += SUBS)
+                        taps4<decltype(count)::value>(part, sc.window(step, g * a.W + r, local), w + r * sp, a.S);
+                });
+                const float c = deal4<NT>(part);
+                if (lane % 16 < QUADS && key + lane / 16 < end) out[(int64_t)g * m.span + lane / 16] = c * a.scale;
+            } else {
+                for (int j0 = sub * JB; j0 < m.R2; j0 += SUBS * JB) {
+                    float c[JB][4];
 #pragma unroll
-                for (int u = 0; u < JB; ++u) c[u] = 0.0f;
-                const int i_end = j0 + JB + a.R - 1 < a.W ? j0 + JB + a.R - 1 : a.W;
-                for (int i = j0; i < i_end; ++i) {
-                    const float *x = x0 + (g * a.W + i) * sc.stride;
-                    for (int t = sub; t < a.S; t += SUBS) {
-                        const float v = x[t];
+                    for (int u = 0; u < JB; ++u) c[u][0] = c[u][1] = c[u][2] = c[u][3] = 0.0f;
+                    with_taps(a.S, [&](auto count) {
+                        for (int i = 0; i < a.R + JB - 1; ++i) {
+                            // (behind the last row there are outputs that nobody writes)
+                            const float *x = sc.window(step, g * a.W + (j0 + i < a.W ? j0 + i : a.W - 1), local);
 #pragma unroll
-                        for (int u = 0; u < JB; ++u) {
-                            const int r = i - j0 - u;
-                            if (r >= 0 && r < a.R) c[u] = fmaf(weights[(g * a.R + r) * sp + t], v, c[u]);   // (wavefront-uniform)
+                            for (int u = 0; u < JB; ++u)
+                                if (i - u >= 0 && i - u < a.R) taps4<decltype(count)::value>(c[u], x, w + (i - u) * sp, a.S);   // (wavefront-uniform)
                         }
-                    }
-                }
+                    });
 #pragma unroll
-                for (int u = 0; u < JB; ++u) {
-                    if constexpr (SUBS >= 2) c[u] = across32(c[u], [](float p, float q) { return p + q; });
-                    if constexpr (SUBS == 4) c[u] = across16(c[u], [](float p, float q) { return p + q; });
-                    if (j0 + u < m.R2 && sub == 0 && key < end)
-                        m.s1[(((int64_t)b * a.heads + h0 + g) * m.R2 + j0 + u) * m.span + (key - s.base)] = c[u] * a.scale;
+                    for (int u = 0; u < JB; ++u)   // (whole vectors: a row has room for them, and nobody reads behind the last key)
+                        if (j0 + u < m.R2 && key < end)
+                            *reinterpret_cast<f32x4 *>(out + ((int64_t)g * m.R2 + j0 + u) * m.span) = f32x4{c[u][0], c[u][1], c[u][2], c[u][3]} * a.scale;
                 }
             }
+        }
     }
 }
 
@@ -306,6 +314,7 @@ template <typename T, int D> __global__ __launch_bounds__(256) void decode_sum_k
     const int splits = (s.n - (s.lo & ~15) + m.v_len - 1) / m.v_len;
     const float *o = m.part + ((int64_t)b * m.d.heads + h) * m.v_splits * D + d;
     float sum = 0.0f;
+#pragma unroll 8
     for (int i = part; i < splits; i += PARTS) sum += o[(int64_t)i * D];
     so[part][d] = sum;
     __syncthreads();
@@ -369,9 +378,9 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
     return MTA_OK;
 }
 
-template <typename T, int D, int NT, int JB> int launch_scores(const mta_args &m, const plan &p, hipStream_t st)
+template <typename T, int D, int NT, int JB, bool ONE> int launch_scores(const mta_args &m, const plan &p, hipStream_t st)
 {
-    auto kern = decode_scores_kernel<T, D, NT, JB>;
+    auto kern = decode_scores_kernel<T, D, NT, JB, ONE>;
     if (const int e = allow_lds(kern, p.lds)) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)p.n_splits, (unsigned)(m.d.heads / p.gw), (unsigned)m.d.slots), dim3(256), p.lds, st, m);
     return launch_status();
@@ -388,12 +397,17 @@ template <typename T, int D, int NT, bool POST> int launch_values_heads(const mt
     return p.v_gw == 4 ? launch_values<T, D, NT, 4, POST>(m, p, st) : p.v_gw == 2 ? launch_values<T, D, NT, 2, POST>(m, p, st)
                                                                                    : launch_values<T, D, NT, 1, POST>(m, p, st);
 }
+template <typename T, int D, int NT> int launch_scores_rows(const mta_args &m, const plan &p, hipStream_t st)
+{
+    constexpr int SUBS = 16 / NT;
+    return m.R2 == 1 ? launch_scores<T, D, NT, 1, true>(m, p, st) : m.R2 <= SUBS ? launch_scores<T, D, NT, 1, false>(m, p, st)
+         : m.R2 <= 2 * SUBS ? launch_scores<T, D, NT, 2, false>(m, p, st) : launch_scores<T, D, NT, 3, false>(m, p, st);
+}
 template <typename T, int D> int launch_all(const mta_args &m, const plan &p, hipStream_t st)
 {
     constexpr int WIDE = D * (int)sizeof(T) > 256 ? 2 : 4;
     const unsigned slots = (unsigned)m.d.slots, heads = (unsigned)m.d.heads;
-    int e = m.R2 == 1 ? (p.nt == 1 ? launch_scores<T, D, 1, 1>(m, p, st) : launch_scores<T, D, WIDE, 1>(m, p, st))
-                      : (p.nt == 1 ? launch_scores<T, D, 1, 4>(m, p, st) : launch_scores<T, D, WIDE, 4>(m, p, st));
+    int e = p.nt == 1 ? launch_scores_rows<T, D, 1>(m, p, st) : launch_scores_rows<T, D, WIDE>(m, p, st);
     if (e) return e;
     if ((e = allow_lds(decode_mix_kernel, p.mix_lds))) return e;
     hipLaunchKernelGGL(decode_mix_kernel, dim3((unsigned)p.chunks, (unsigned)m.R2, slots), dim3(256), p.mix_lds, st, m);
@@ -442,7 +456,7 @@ extern "C" int mta_decode(const mta_cache *c, const void *w, const void *w_pre, 
     if (!w || !o || !workspace || (!w2 && (R2 != 1 || S2 != 1))) return MTA_ERR_NULL;
     const int ws = dtype_size(w_dtype);
     if (ws == 0) return MTA_ERR_DTYPE;
-    if (!aligned_to(w, ws) || !aligned_to(w_pre, ws) || !aligned_to(w2, ws) || !aligned_to(w_post, ws) || !aligned_to(o, dtype_size(c->dtype)) || !aligned_to(workspace, 8))
+    if (!aligned_to(w, ws) || !aligned_to(w_pre, ws) || !aligned_to(w2, ws) || !aligned_to(w_post, ws) || !aligned_to(o, dtype_size(c->dtype)) || !aligned_to(workspace, 16))
         return MTA_ERR_ALIGN;
     mta_args m = {};
     m.pre_group = !w_pre ? 1 : pre_group ? pre_group : c->heads;
