@@ -32,7 +32,7 @@ struct decode_args {
     int slots, max_pages, page_shift, heads, kv_heads, share, ring;
     int R, S, W;                // conv kernel; query rows of raw scores (R + output rows - 1)
     int w_dtype, window, longest;
-    int split_len, n_splits;    // keys per split; splits that the grid and the workspace have room for
+    int target, least, items;   // how the slots' keys are shared out (shares)
     int gw;                     // query heads per workgroup
     float scale;
 };
@@ -101,6 +101,103 @@ template <int STEP> __device__ __forceinline__ float lanes_sum(float v)
     return v;
 }
 
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_or_0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true); }
+// the sum over the lanes up to this one: within rows of 16, then the rows' last sums onto the rows behind them
+__device__ __forceinline__ int wave_scan(int v)
+{
+    v += dpp_or_0<0x111, 0xf>(v);
+    v += dpp_or_0<0x112, 0xf>(v);
+    v += dpp_or_0<0x114, 0xf>(v);
+    v += dpp_or_0<0x118, 0xf>(v);
+    v += dpp_or_0<0x142, 0xa>(v);
+    v += dpp_or_0<0x143, 0xc>(v);
+    return v;
+}
+
+// How the slots' keys are shared out over workgroups.  The host knows the longest slot at most (a captured graph: not even that), so the
+// device does it: every slot's keys in steps of `ch`, `per` steps to an item.  Items of one size, however different the lengths, and all that live
+// next to each other in the grid, which deals its workgroups over the XCDs in turn: with a grid of (split, head, slot) short slots left
+// whole XCDs idle (conv-attention, 16 slots of 1k to 8k keys 204 us, now 153; MTA, 16 slots of 512 to 4k keys 142, now 84).
+// per: `target` items are one round of workgroups that are all resident (an item costs some 5 us beside its keys - the table, queries, weights,
+// the first loads, the results - which a second round pays again: 8k keys of 32 heads 30 us in one round, 37 in two); where they come
+// out long, four times as many, which even out the end (16 slots of up to 8k keys 165 us in items of 25 steps, 153 in 7).
+// A slot has an item at least: somebody writes its result.  Every wavefront computes this for itself, a slot to a lane.
+struct shares {
+    const decode_args &a;
+    int older, ch, per;
+    bool newest;                // the keys of the newest row only, not of all output rows
+    static constexpr int LONG = 8, SHORT = 6, MORE = 4;
+
+    __device__ __forceinline__ int from(const slot_step &s) const { return newest ? s.lo & ~15 : s.base; }
+    __device__ __forceinline__ int steps(const slot_step &s) const { return s.n > 0 ? (s.n - from(s) + ch - 1) / ch : 0; }
+    __device__ __forceinline__ slot_step slot(int b) const
+    {
+        slot_step s = {0, 0, 0};
+        if (b < a.slots) s = step_of(a, b, older);
+        return s;
+    }
+    __device__ __forceinline__ shares(const decode_args &a_, int older_, int ch_, bool newest_, int lane) : a(a_), older(older_), ch(ch_), newest(newest_)
+    {
+        float total = 0.0f;     // (of up to 2^40 steps; the same in every wavefront)
+        for (int b0 = 0; b0 < a.slots; b0 += 64) total += (float)steps(slot(b0 + lane));
+        total = wave_sum(total);
+        per = (int)ceilf(total / (float)a.target);
+        if (per > LONG) {
+            per = (int)ceilf(total / (float)(MORE * a.target));
+            if (per < SHORT) per = SHORT;
+        }
+        if (per < a.least) per = a.least;
+    }
+    // the items of 64 slots from b0 on, one slot to a lane
+    __device__ __forceinline__ int items(int b, const slot_step &s) const
+    {
+        const int n = (steps(s) + per - 1) / per;
+        return b >= a.slots ? 0 : n > 1 ? n : 1;
+    }
+};
+// Item `index`: its slot's step, the slot's first item and their number; slot < 0: there is no such item.
+struct work_item { slot_step s; int slot, first, count; };
+__device__ __forceinline__ work_item item_of(const shares &sh, int index, int lane)
+{
+    work_item w;
+    int before = 0;
+    for (int b0 = 0; b0 < sh.a.slots; b0 += 64) {
+        const slot_step s = sh.slot(b0 + lane);
+        const int n = sh.items(b0 + lane, s), upto = before + wave_scan(n);
+        const uint64_t behind = __ballot(upto > index);
+        if (behind) {
+            const int l = __builtin_ctzll(behind);
+            w.slot = b0 + l;
+            w.count = __builtin_amdgcn_readlane(n, l);
+            w.first = __builtin_amdgcn_readlane(upto, l) - w.count;
+            w.s.n = __builtin_amdgcn_readlane(s.n, l), w.s.base = __builtin_amdgcn_readlane(s.base, l), w.s.lo = __builtin_amdgcn_readlane(s.lo, l);
+            return w;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+    w.slot = -1;
+    return w;
+}
+// ... and the items of a slot
+__device__ __forceinline__ work_item items_of(const shares &sh, int slot, int lane)
+{
+    work_item w;
+    int before = 0;
+    for (int b0 = 0;; b0 += 64) {
+        const slot_step s = sh.slot(b0 + lane);
+        const int n = sh.items(b0 + lane, s), upto = before + wave_scan(n);
+        if (slot < b0 + 64) {
+            const int l = slot - b0;
+            w.slot = slot;
+            w.count = __builtin_amdgcn_readlane(n, l);
+            w.first = __builtin_amdgcn_readlane(upto, l) - w.count;
+            w.s.n = __builtin_amdgcn_readlane(s.n, l), w.s.base = __builtin_amdgcn_readlane(s.base, l), w.s.lo = __builtin_amdgcn_readlane(s.lo, l);
+            return w;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+
 // c += a b^T over 64 bytes of 16 rows each; a lane holds 16 bytes of row lane % 16.  (Which of the contracted elements a lane group holds is
 // the same for both operands, so any order of them will do: rows of fp32 are read 16 bytes per lane as well and take four 16x16x4 steps.)
 template <typename T> __device__ __forceinline__ void mma_rows(f32x4 &c, const u32x4 &a, const u32x4 &b);
@@ -160,11 +257,39 @@ __host__ __device__ __forceinline__ raw_layout raw_layout_of(int rows, int R, in
     return l;
 }
 
+// 64 entries of a slot's row of the table, one per lane, from the page of `key` on: one load and one wait for all the tiles they serve.  (An entry
+// at a time was a chain of waits ahead of the first loads of K and V: 14k of a workgroup's 31k cycles at 8k keys of 32 heads.)
+struct page_map {
+    int first, entry;
+    __device__ __forceinline__ void load(const decode_args &a, int b, int key, int lane)
+    {
+        first = (key > 0 ? key : 0) >> a.page_shift;
+        const int i = first + lane;
+        entry = a.table[(int64_t)b * a.max_pages + (i < a.max_pages ? i : a.max_pages - 1)];
+    }
+    // ... from the page of `key` on, if those up to that of `last` are not there
+    __device__ __forceinline__ void reach(const decode_args &a, int b, int key, int last, int lane)
+    {
+        if ((last >> a.page_shift) - first >= 64) load(a, b, key, lane);
+    }
+    // Where a lane's bytes (at `offset` from the tile's first row of ROW bytes) of the tile at key0 lie in a pool.  Of a tile that is not wanted, or
+    // whose entry names no page (ok = false), all lanes get the pool's first bytes, which the caller does not use: loads without branches
+    // around them stay in flight behind each other (with branches the wait for one was a wait for all), and one line costs next to nothing.
+    template <int ROW> __device__ __forceinline__ const char *tile(const decode_args &a, int kvh, const char *pool, int key0, int offset, bool wanted, bool &ok) const
+    {
+        const int e = __builtin_amdgcn_readlane(entry, wanted ? (key0 >> a.page_shift) - first : 0);
+        ok = (unsigned)e < (uint64_t)a.n_pages;
+        const bool there = ok && wanted;
+        const int64_t block = there ? (int64_t)e * a.kv_heads + kvh : 0;
+        return pool + ((block << a.page_shift) + (there ? key0 & ((1 << a.page_shift) - 1) : 0)) * ROW + (there ? offset : 0);
+    }
+};
+
 // The rows' raw scores, step by step.
 template <typename T, int D, int NT> struct raw_scores {
     static constexpr int ROW = D * (int)sizeof(T), NC = ROW / 64, CH = 64 * NT;
     const decode_args &a;
-    const int *entries;         // the slot's row of the table
+    page_map pages;
     unsigned char *qs;          // query rows in LDS
     int *pos;                   // their positions
     float *raw;
@@ -172,39 +297,22 @@ template <typename T, int D, int NT> struct raw_scores {
     u32x4 kreg[NT][NC];
     int bad;                    // bit t: tile t lies in a page that is none
 
-    __device__ __forceinline__ raw_scores(const decode_args &a_, unsigned char *smem, const raw_layout &l, int rows_, int b, int kvh_, int n_, int limit_)
-        : a(a_), entries(a_.table + (int64_t)b * a_.max_pages), qs(smem), pos(reinterpret_cast<int *>(smem + up16(rows_) * q_stride(ROW))),
+    __device__ __forceinline__ raw_scores(const decode_args &a_, unsigned char *smem, const raw_layout &l, const page_map &pages_, int rows_, int kvh_, int n_, int limit_)
+        : a(a_), pages(pages_), qs(smem), pos(reinterpret_cast<int *>(smem + up16(rows_) * q_stride(ROW))),
           raw(reinterpret_cast<float *>(smem + l.raw)), rows(rows_), n(n_), limit(limit_), kvh(kvh_), lane((int)threadIdx.x & 63),
           wave(__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6)), hl(halo_left(a_.S)), hr(halo_right(a_.S)), stride(raw_stride(a_.S, NT)), bad(0)
     {
     }
 
-    // where the rows of one 16-key tile begin in a pool; nullptr: in no page
-    __device__ __forceinline__ const char *tile(const char *pool, int key0) const
+    // A tile of keys, if it holds any that this split needs; false: it lies in no page.
+    __device__ __forceinline__ bool load(u32x4 (&dst)[NC], int key0, bool wanted = true) const
     {
-        const int entry = entries[key0 >> a.page_shift];
-        if ((unsigned)entry >= (uint64_t)a.n_pages) return nullptr;
-        const int64_t block = (int64_t)entry * a.kv_heads + kvh;
-        return pool + (((block << a.page_shift) + (key0 & ((1 << a.page_shift) - 1))) * ROW);
-    }
-    // A tile of keys; nothing is read of one that holds none of the keys this split needs.
-    __device__ __forceinline__ bool load(u32x4 (&dst)[NC], int key0) const
-    {
-        if (key0 < 0 || key0 >= limit) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) dst[c] = u32x4{0, 0, 0, 0};
-            return true;
-        }
-        const char *at = tile(a.k, key0);
-        if (!at) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) dst[c] = u32x4{0, 0, 0, 0};
-            return false;
-        }
-        at += (lane & 15) * ROW + (lane >> 4) * 16;
+        bool ok;
+        wanted = wanted && key0 >= 0 && key0 < limit;
+        const char *at = pages.tile<ROW>(a, kvh, a.k, key0, (lane & 15) * ROW + (lane >> 4) * 16, wanted, ok);
 #pragma unroll
         for (int c = 0; c < NC; ++c) dst[c] = *reinterpret_cast<const u32x4 *>(at + 64 * c);
-        return true;
+        return ok || !wanted;
     }
     __device__ __forceinline__ int first_of(int kb, int t) const { return kb + hr + (wave * NT + t) * 16; }   // (a step's new keys)
     __device__ __forceinline__ void load_step(int kb)
@@ -220,7 +328,8 @@ template <typename T, int D, int NT> struct raw_scores {
         const int group = lane >> 4, at = lane & 15;
         // (all rows see all of these keys: nothing to replace)
         const bool plain = is_bad == 0 && a.window == 0 && key0 >= 0 && key0 + 16 * N - 1 <= n - a.W;
-        for (int m0 = 0; m0 < rows; m0 += 16) {
+        int m0 = 0;
+        do {   // (at least once, which the compiler has to know to keep other loads in flight)
             f32x4 acc[N];
 #pragma unroll
             for (int t = 0; t < N; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -257,36 +366,55 @@ template <typename T, int D, int NT> struct raw_scores {
                         if (col + 16 * t >= CH) next[(r0 + v) * stride + col + 16 * t - CH + at] = acc[t][v];
                 }
             }
-        }
+        } while ((m0 += 16) < rows);
     }
     __device__ __forceinline__ float *buffer(int step) const { return raw + raw_shift(a.S) + (step % 3) * rows * stride; }
-    // Query rows, their positions and the conv weights into LDS: rows g * W + i, position p - W + 1 + i of query head h0 + g.
-    __device__ __forceinline__ void stage(unsigned char *smem, const raw_layout &l, int b, int h0) const
+    // What precedes the first step.  begin(): the loads of the tiles ahead of its new keys (one per wavefront at most, four at S = 63), of the query
+    // rows and of the weights, ahead of the first step's own; finish(): query rows (g * W + i: position p - W + 1 + i of query head h0 + g), their
+    // positions and weights to LDS, and the scores of those tiles.
+    struct start {
+        u32x4 halo[1][NC], q[2];
+        float w[2];
+        bool halo_ok;
+    };
+    __device__ __forceinline__ int position(int r) const { return r < rows ? n - a.W + r % a.W : -1; }
+    __device__ __forceinline__ u32x4 query(int x, int b, int h0) const
     {
-        const int padded = up16(rows), W = a.W;
-        for (int x = threadIdx.x; x < padded * (ROW / 16); x += 64 * DECODE_WAVES) {
-            const int r = x / (ROW / 16), c = x % (ROW / 16), g = r / W, p = n - W + (r - g * W);
-            u32x4 val = {0, 0, 0, 0};
-            if (r < rows && p >= 0)
-                val = *reinterpret_cast<const u32x4 *>(a.q + (((int64_t)b * a.heads + h0 + g) * a.ring + p % a.ring) * ROW + 16 * c);
-            *reinterpret_cast<u32x4 *>(qs + r * q_stride(ROW) + 16 * c) = val;
-            if (c == 0) pos[r] = r < rows ? p : -1;
-        }
-        float *w = reinterpret_cast<float *>(smem + l.weights);
-        const int sp = (a.S + 3) & ~3, taps = a.R * a.S;
-        for (int x = threadIdx.x; x < a.gw * taps; x += 64 * DECODE_WAVES) {
-            const int g = x / taps, r = (x - g * taps) / a.S, s = x - g * taps - r * a.S;
-            w[(g * a.R + r) * sp + s] = load_any(a.w, a.w_dtype, (int64_t)(h0 + g) * taps + r * a.S + s);
+        const int r = x / (ROW / 16), c = x % (ROW / 16), g = r / a.W, p = position(r);
+        u32x4 val = {0, 0, 0, 0};
+        if (p >= 0) val = *reinterpret_cast<const u32x4 *>(a.q + (((int64_t)b * a.heads + h0 + g) * a.ring + p % a.ring) * ROW + 16 * c);
+        return val;
+    }
+    __device__ __forceinline__ void begin(start &st, int kb, int b, int h0) const
+    {
+        const int taps = a.gw * a.R * a.S, tid = threadIdx.x;
+        const int64_t w0 = (int64_t)h0 * a.R * a.S;
+        st.halo_ok = load(st.halo[0], kb - hl + wave * 16, wave * 16 < hl + hr);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            st.q[u] = query(tid + 256 * u, b, h0);
+            st.w[u] = load_any(a.w, a.w_dtype, w0 + (tid + 256 * u < taps ? tid + 256 * u : 0));
         }
     }
-    // the tiles ahead of the first step's new keys: one per wavefront at most (four at S = 63)
-    __device__ __forceinline__ void halo(int kb) const
+    __device__ __forceinline__ void finish(const start &st, int kb, int b, int h0, unsigned char *smem, const raw_layout &l) const
     {
-        if (wave * 16 >= hl + hr) return;
-        u32x4 kr[1][NC];
-        const int key0 = kb - hl + wave * 16;
-        const bool ok = load(kr[0], key0);
-        score<1>(kr, key0, !ok, buffer(0), wave * 16, nullptr);
+        const int vecs = up16(rows) * (ROW / 16), taps = a.gw * a.R * a.S, sp = (a.S + 3) & ~3, tid = threadIdx.x;
+        const int64_t w0 = (int64_t)h0 * a.R * a.S;
+        float *const w = reinterpret_cast<float *>(smem + l.weights);
+        auto put = [&](int x, const u32x4 &val, int p) {
+            *reinterpret_cast<u32x4 *>(qs + x / (ROW / 16) * q_stride(ROW) + x % (ROW / 16) * 16) = val;
+            if (x % (ROW / 16) == 0) pos[x / (ROW / 16)] = p;
+        };
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int x = tid + 256 * u;
+            if (x < vecs) put(x, st.q[u], position(x / (ROW / 16)));
+            if (x < taps) w[x / a.S * sp + x % a.S] = st.w[u];
+        }
+        for (int x = tid + 512; x < vecs; x += 256) put(x, query(x, b, h0), position(x / (ROW / 16)));
+        for (int x = tid + 512; x < taps; x += 256) w[x / a.S * sp + x % a.S] = load_any(a.w, a.w_dtype, w0 + x);
+        __syncthreads();
+        if (wave * 16 < hl + hr) score<1>(st.halo, kb - hl + wave * 16, !st.halo_ok, buffer(0), wave * 16, nullptr);
     }
     // this step's scores, from the keys that load_step() brought
     __device__ __forceinline__ void score_step(int kb, int step) const
@@ -347,19 +475,45 @@ template <typename F> __device__ __forceinline__ void with_taps(int S, F f)
     default: f(count_of<0>()); break;
     }
 }
-// Four values per lane, for the keys 4 * (lane % (4 NT)) .. + 3, partial over the lanes of equal lane % (4 NT): the whole sum of key
-// 4 * (lane % (4 NT)) + lane / 16 in every lane.  Halves and rows change places as they are added, so a value is moved once and not four times.
-template <int NT> __device__ __forceinline__ float deal4(float (&c)[4])
-{
-    swap32(c[0], c[2]);
-    swap32(c[1], c[3]);
-    uint32_t p = __float_as_uint(c[0] + c[2]), q = __float_as_uint(c[1] + c[3]);   // lower half: keys 0 and 1, upper half: 2 and 3
-    swap16(p, q);
-    float v = __uint_as_float(p) + __uint_as_float(q);
-    if constexpr (NT <= 2) v += dpp<0x128>(v);
-    if constexpr (NT == 1) v += dpp<0x124>(v);
-    return v;
-}
+// How a wavefront's 64 lanes share 16 NT keys of GW heads, four keys to a lane: quad (4 NT of them), head, and the rows of taps, dealt over RG
+// lanes.  deal() adds the RG parts and leaves each lane VALUES whole sums, of keys first .. first + VALUES - 1 of its quad: halves and rows of
+// lanes change places as they are added, so a value is moved once.  With RG > 4 several lanes hold the same key, one of them is its owner.
+template <int NT, int GW> struct score_lanes {
+    static constexpr int QUADS = 4 * NT, RG = 16 / (NT * GW), VALUES = RG == 1 ? 4 : RG == 2 ? 2 : 1;
+    int quad, head, part, key;
+    bool owner;
+    __device__ __forceinline__ explicit score_lanes(int lane)
+        : quad(lane % QUADS), head(lane / QUADS % GW), part(lane / (QUADS * GW)),
+          key(4 * (lane % QUADS) + (RG == 1 ? 0 : RG == 2 ? 2 * (lane >> 5) : lane >> 4)), owner(RG <= 4 || lane / (QUADS * GW) % (RG / 4 + (RG < 4)) == 0)
+    {
+    }
+    __device__ __forceinline__ void deal(float (&c)[4]) const
+    {
+        if constexpr (RG >= 2) {
+            swap32(c[0], c[2]);
+            swap32(c[1], c[3]);
+            c[0] += c[2], c[1] += c[3];   // lower half: keys 0 and 1, upper half: 2 and 3
+        }
+        if constexpr (RG >= 4) {
+            uint32_t p = __float_as_uint(c[0]), q = __float_as_uint(c[1]);
+            swap16(p, q);
+            c[0] = __uint_as_float(p) + __uint_as_float(q);
+        }
+        if constexpr (RG >= 8) c[0] += dpp<0x128>(c[0]);
+        if constexpr (RG == 16) c[0] += dpp<0x124>(c[0]);
+    }
+    // over all lanes of the same head
+    template <typename F> __device__ __forceinline__ static float reduce(float v, F op)
+    {
+        v = op(v, dpp<0xb1>(v));
+        v = op(v, dpp<0x4e>(v));
+        if constexpr (!(QUADS == 4 && GW >= 2)) v = op(v, dpp<0x141>(v));
+        if constexpr (!((QUADS == 4 && GW == 4) || (QUADS == 8 && GW >= 2))) v = op(v, dpp<0x128>(v));
+        if constexpr (!((QUADS == 8 && GW == 4) || (QUADS == 16 && GW >= 2))) v = across16(v, op);
+        if constexpr (!(QUADS == 16 && GW == 4)) v = across32(v, op);
+        return v;
+    }
+};
 
 // A wavefront's 16 * NT rows of V times the probabilities of GW heads: a row is read by ROW / 16 lanes.
 template <typename T, int D, int NT, int GW> struct value_rows {
@@ -374,25 +528,29 @@ template <typename T, int D, int NT, int GW> struct value_rows {
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[g][e] = 0.0f;
     }
-    // rows first .. first + 16 NT - 1; zeros for those outside lo .. end - 1.  tile(key) gives a tile's place, or nullptr
-    template <typename F> __device__ __forceinline__ void load(int first, int lo, int end, int lane, F tile)
+    // rows first .. first + 16 NT - 1, as far as they lie in lo .. end - 1
+    __device__ __forceinline__ void load(const decode_args &a, const page_map &pages, int kvh, int first, int lo, int end, int lane)
     {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            bool ok;
             const int key0 = first + 16 * t;
-            const char *at = key0 < end && key0 + 15 >= lo ? tile(key0) : nullptr;
+            const char *at = pages.tile<ROW>(a, kvh, a.v, key0, lane / LPR * ROW + lane % LPR * 16, key0 < end && key0 + 15 >= lo, ok);
 #pragma unroll
-            for (int i = 0; i < 16 / RPI; ++i) {
-                const int row = i * RPI + lane / LPR;
-                u32x4 x = {0, 0, 0, 0};
-                if (at && key0 + row >= lo && key0 + row < end) x = *reinterpret_cast<const u32x4 *>(at + row * ROW + (lane % LPR) * 16);
-                vreg[t * (16 / RPI) + i] = x;
-            }
+            for (int i = 0; i < 16 / RPI; ++i) vreg[t * (16 / RPI) + i] = *reinterpret_cast<const u32x4 *>(at + i * RPI * ROW);
+            // (a page that is none: its keys' probabilities are NaN)
         }
     }
-    // probs: the wavefront's rows, 16 NT of each head
-    __device__ __forceinline__ void multiply(const float *probs, int lane)
+    // the same rows times probs, 16 NT of each head
+    __device__ __forceinline__ void multiply(const float *probs, int first, int lo, int end, int lane)
     {
+        if (first < lo || first + 16 * NT > end) {   // (replaced, not multiplied by 0: what lies there may be anything)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int key = first + i * RPI + lane / LPR;
+                if (key < lo || key >= end) vreg[i] = u32x4{0, 0, 0, 0};
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const wide<T> x = widen<T>(vreg[i]);
@@ -452,11 +610,35 @@ inline int64_t span_of(int64_t longest, int window, int out_rows)
     const int64_t seen = window > 0 ? (int64_t)window + out_rows - 1 + 15 : longest;
     return seen < longest ? seen : longest;
 }
+// Keys per step and wavefront, in tiles of 16: 8 KB of K and as many of V.  More in flight is slower, not faster: a kernel that only reads pages
+// this way gets 5.8 to 6.1 TB/s with one or two tiles of 256-byte rows and 4.6 with four, whatever the number of workgroups.
+constexpr int most_tiles(int row_bytes) { return row_bytes >= 512 ? 1 : 512 / row_bytes; }
+// Keys per step (64 nt, nt up to `most`), and what `shares` goes by; `groups` workgroups take an item, one of them for some heads each.  Two
+// workgroups to a CU are one round, four of the shortest steps, which fewer than four of the longer ones would not fill.
+struct cut { int nt, target, least, items; bool joined; };
+inline cut cut_of(int64_t span, int64_t slots, int64_t groups, int most)
+{
+    cut c = {};
+    for (c.nt = most; c.nt >= 1; c.nt >>= 1) {
+        const int64_t steps = (span + 64 * c.nt - 1) / (64 * c.nt), resident = c.nt == 1 ? 1024 : 512;
+        c.target = (int)(resident / groups > 1 ? resident / groups : 1);
+        if (c.nt > 1 && steps * slots < 4 * c.target) continue;
+        c.least = c.nt == 1 ? 1 : 2;
+        c.joined = steps > c.least;   // (else no slot has more than one item)
+        const int64_t most_items = (steps * slots > (int64_t)shares::LONG * c.target ? shares::MORE * c.target : c.target) + slots + 1;
+        const int64_t all = slots * ((steps + c.least - 1) / c.least);
+        c.items = (int)(all < most_items ? all : most_items);
+        break;
+    }
+    return c;
+}
 template <typename K> inline int allow_lds(K kern, int bytes)
 {
     if (bytes <= 64 << 10) return MTA_OK;
     const hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     return e == hipSuccess ? MTA_OK : (int)e;
 }
+// (a launch has fewer than 2^32 threads)
+inline bool too_many(const cut &c, int64_t groups) { return c.items * groups >= 1 << 24; }
 
 }  // namespace mta

@@ -8,94 +8,111 @@
 namespace mta {
 namespace {
 
-// The results of a split: per (slot, head, split) a row of D sums, then {reference, sum of exponentials}.
-__host__ __device__ __forceinline__ int64_t stats_offset(int64_t slots, int64_t heads, int64_t splits, int D) { return slots * heads * splits * D; }
+// The results of an item: per (item, head) a row of D sums, then {reference, sum of exponentials}.
+__host__ __device__ __forceinline__ int64_t stats_offset(int64_t items, int64_t heads, int D) { return items * heads * D; }
 
 template <typename T, int D, int NT, int GW>
-__global__ __launch_bounds__(256) void conv_attn_decode_kernel(const decode_args a)
+__global__ __launch_bounds__(256, 2) void conv_attn_decode_kernel(const decode_args a)
 {
     extern __shared__ __align__(16) unsigned char smem[];
-    const int b = blockIdx.z, h0 = blockIdx.y * GW, split = blockIdx.x, tid = threadIdx.x;
+    constexpr int CH = 64 * NT;
+    const int tid = threadIdx.x, lane = tid & 63, groups = a.heads / GW, index = blockIdx.x / groups, h0 = (blockIdx.x - index * groups) * GW;
+    const shares sh(a, 0, CH, false, lane);
+    const work_item it = item_of(sh, index, lane);
+    if (it.slot < 0) return;
+    const slot_step s = it.s;
+    const int b = it.slot;
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h0) * D;
-    const slot_step s = step_of(a, b, 0);
     if (s.n <= 0) {
-        if (a.n_splits == 1)   // (else the join says so)
-            for (int x = tid; x < GW * D; x += 256) out[x] = from_float<T>(s.n < 0 ? __builtin_nanf("") : 0.0f);
+        for (int x = tid; x < GW * D; x += 256) out[x] = from_float<T>(s.n < 0 ? __builtin_nanf("") : 0.0f);
         return;
     }
-    const int beg = s.base + split * a.split_len;
-    if (beg >= s.n) return;
-    const int end = beg + a.split_len < s.n ? beg + a.split_len : s.n;
+    const int beg = s.base + (index - it.first) * sh.per * CH, end = beg + sh.per * CH < s.n ? beg + sh.per * CH : s.n;
+    page_map pages;
+    pages.load(a, b, beg - halo_left(a.S), lane);
 
-    constexpr int CH = 64 * NT, QUADS = 4 * NT, SUBS = 64 / QUADS;   // (four keys per lane, a key's rows of taps dealt over SUBS lanes)
-    const int rows = GW * a.R, left = (a.S - 1) / 2, reach = end + a.S - 1 - left;
+    using lanes = score_lanes<NT, GW>;
+    const int rows = GW * a.R, right = a.S - 1 - (a.S - 1) / 2;
     const raw_layout l = raw_layout_of(rows, a.R, a.S, GW, D, (int)sizeof(T), NT, true);
-    raw_scores<T, D, NT> sc(a, smem, l, rows, b, h0 / a.share, s.n, reach < s.n ? reach : s.n);
-    const int lane = sc.lane, wave = sc.wave, quad = lane % QUADS, sub = lane / QUADS, mine = 4 * quad + lane / 16;
-    const bool owner = lane % 16 < QUADS;   // (with NT < 4 several lanes come to hold the same key)
-    const float *const weights = reinterpret_cast<const float *>(smem + l.weights);
+    raw_scores<T, D, NT> sc(a, smem, l, pages, rows, h0 / a.share, s.n, end + right < s.n ? end + right : s.n);
+    const int wave = sc.wave, sp = (a.S + 3) & ~3;
+    const lanes me(lane);
+    const float *const weights = reinterpret_cast<const float *>(smem + l.weights) + me.head * a.R * sp;
     float *const probs = reinterpret_cast<float *>(smem + l.probs) + wave * GW * 16 * NT;
-    const int sp = (a.S + 3) & ~3;
     const float scale2 = a.scale * LOG2E;
 
-    sc.load_step(beg);
-    sc.stage(smem, l, b, h0);
-    __syncthreads();
-    sc.halo(beg);
-
+    // K and V are always under way a step ahead
     value_rows<T, D, NT, GW> val;
+    typename raw_scores<T, D, NT>::start st;
+    sc.begin(st, beg, b, h0);
+    sc.load_step(beg);
+    val.load(a, sc.pages, sc.kvh, beg + wave * 16 * NT, s.lo, end, lane);
     val.clear();
-    float m[GW], sum[GW];
-#pragma unroll
-    for (int g = 0; g < GW; ++g) m[g] = -INFINITY, sum[g] = 0.0f;
+    sc.finish(st, beg, b, h0, smem, l);
 
-    int step = 0;
-    for (int kb = beg; kb < end; kb += CH, ++step) {
+    float m = -INFINITY, sum = 0.0f;   // a lane's head: reference, and its own keys' sum
+    auto advance = [&](int kb, int step, auto more) {
         const int first = kb + wave * 16 * NT;
-        val.load(first, s.lo, end, lane, [&](int key0) { return sc.tile(a.v, key0); });
         sc.score_step(kb, step);
-        if (kb + CH < end) sc.load_step(kb + CH);
+        if constexpr (more.value) {
+            sc.pages.reach(a, b, kb + CH, kb + 2 * CH + sc.hr < sc.limit ? kb + 2 * CH + sc.hr : sc.limit, lane);
+            sc.load_step(kb + CH);
+        }
         __syncthreads();
-        const int key = first + mine;
-        const bool seen = key >= s.lo && key < end;
+        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        with_taps(a.S, [&](auto count) {
+            for (int r = me.part; r < a.R; r += lanes::RG)
+                taps4<decltype(count)::value>(c, sc.window(step, me.head * a.R + r, wave * 16 * NT + 4 * me.quad), weights + r * sp, a.S);
+        });
+        me.deal(c);
+        float top = m;
+        bool seen[lanes::VALUES];
 #pragma unroll
-        for (int g = 0; g < GW; ++g) {
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            with_taps(a.S, [&](auto count) {
-                for (int r = sub; r < a.R; r += SUBS)
-                    taps4<decltype(count)::value>(part, sc.window(step, g * a.R + r, wave * 16 * NT + 4 * quad), weights + (g * a.R + r) * sp, a.S);
-            });
-            const float c = deal4<NT>(part);
-            const float e = seen ? c * scale2 : -INFINITY;
-            const float top = fmaxf(m[g], wave_max(e));
-            if (top > m[g]) {   // (wavefront-uniform)
-                const float fade = exp2f(m[g] - top);
-                m[g] = top;
-                sum[g] *= fade;
+        for (int u = 0; u < lanes::VALUES; ++u) {
+            const int key = first + me.key + u;
+            seen[u] = key >= s.lo && key < end;
+            c[u] = seen[u] ? c[u] * scale2 : -INFINITY;
+            top = fmaxf(top, c[u]);
+        }
+        top = lanes::reduce(top, [](float x, float y) { return fmaxf(x, y); });
+        if (__any(top > m)) {
+            const float fade = m < top ? exp2f(m - top) : 1.0f;
+            m = top;
+            sum *= fade;
 #pragma unroll
-                for (int u = 0; u < val.E; ++u) val.acc[g][u] *= fade;
+            for (int g = 0; g < GW; ++g) {
+                const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(fade), g * lanes::QUADS));
+#pragma unroll
+                for (int u = 0; u < val.E; ++u) val.acc[g][u] *= f;
             }
-            // (no score but -inf so far: a reference of 0, so that such keys count 0 and not NaN)
-            const float p = seen ? __builtin_amdgcn_exp2f(e - (m[g] == -INFINITY ? 0.0f : m[g])) : 0.0f;
-            if (owner) {
-                sum[g] += p;
-                probs[g * 16 * NT + mine] = p;
+        }
+        // (no score but -inf so far: a reference of 0, so that such keys count 0 and not NaN)
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float *const to = probs + me.head * 16 * NT + me.key;
+#pragma unroll
+        for (int u = 0; u < lanes::VALUES; ++u) {
+            const float p = seen[u] ? __builtin_amdgcn_exp2f(c[u] - ref) : 0.0f;
+            if (me.owner) {
+                sum += p;
+                to[u] = p;
             }
         }
         wave_sync();
-        val.multiply(probs, lane);
+        val.multiply(probs, first, s.lo, end, lane);
+        if constexpr (more.value) val.load(a, sc.pages, sc.kvh, first + CH, s.lo, end, lane);
         wave_sync();
-    }
+    };
+    // (the last step apart: a branch around the loads of the others would cost their order)
+    int kb = beg, step = 0;
+    for (; kb + CH < end; kb += CH, ++step) advance(kb, step, count_of<1>());
+    advance(kb, step, count_of<0>());
+    sum = lanes::reduce(sum, [](float x, float y) { return x + y; });
 
     // the four wavefronts' results, brought to one reference
     __syncthreads();
     float *const res = reinterpret_cast<float *>(smem + l.raw), *const ml = res + DECODE_WAVES * GW * D;
     val.store(res + wave * GW * D, lane);
-#pragma unroll
-    for (int g = 0; g < GW; ++g) {
-        const float total = wave_sum(sum[g]);
-        if (lane == 0) ml[(wave * GW + g) * 2] = m[g], ml[(wave * GW + g) * 2 + 1] = total;
-    }
+    if (me.quad == 0 && me.part == 0) ml[(wave * GW + me.head) * 2] = m, ml[(wave * GW + me.head) * 2 + 1] = sum;
     __syncthreads();
     for (int x = tid; x < GW * D; x += 256) {
         const int g = x / D, d = x % D;
@@ -110,43 +127,41 @@ __global__ __launch_bounds__(256) void conv_attn_decode_kernel(const decode_args
             o = fmaf(f, res[(w * GW + g) * D + d], o);
             total = fmaf(f, ml[(w * GW + g) * 2 + 1], total);
         }
-        if (a.n_splits == 1) {
+        if (it.count == 1) {
             out[x] = from_float<T>(o / total);
         } else {
-            const int64_t at = ((int64_t)b * a.heads + h0 + g) * a.n_splits + split;
+            const int64_t at = (int64_t)index * a.heads + h0 + g;
             a.ws[at * D + d] = o;
             if (d == 0) {
-                float *st = a.ws + stats_offset(a.slots, a.heads, a.n_splits, D) + 2 * at;
-                st[0] = top, st[1] = total;
+                float *ml_out = a.ws + stats_offset(a.items, a.heads, D) + 2 * at;
+                ml_out[0] = top, ml_out[1] = total;
             }
         }
     }
 }
 
-// The splits of one (slot, head), brought to one reference and added up, always in the same order.
+// The items of one (slot, head), brought to one reference and added up, always in the same order.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a)
+__global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a, int ch)
 {
     constexpr int PARTS = 256 / D;
     __shared__ float so[PARTS][D], factor[64];
     const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D, lane = threadIdx.x & 63;
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
-    const slot_step s = step_of(a, b, 0);
-    if (s.n <= 0) {
-        if (part == 0) out[d] = from_float<T>(s.n < 0 ? __builtin_nanf("") : 0.0f);
-        return;
-    }
-    const int splits = (s.n - s.base + a.split_len - 1) / a.split_len;
-    const int64_t at = ((int64_t)b * a.heads + h) * a.n_splits;
+    const shares sh(a, 0, ch, false, lane);
+    const work_item it = items_of(sh, b, lane);
+    const int splits = it.count;
+    if (splits == 1) return;   // (that item wrote the result)
+    const int64_t at = (int64_t)it.first * a.heads + h;
     const float *o = a.ws + at * D;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + stats_offset(a.slots, a.heads, a.n_splits, D)) + at;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws + stats_offset(a.items, a.heads, D)) + at;
     float top = -INFINITY;
-    for (int i = lane; i < splits; i += 64) top = fmaxf(top, ml[i].x);
+    for (int i = lane; i < splits; i += 64) top = fmaxf(top, ml[(int64_t)i * a.heads].x);
     top = wave_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, total = 0.0f;
     for (int i0 = 0; i0 < splits; i0 += 64) {   // (factors of 64 splits at a time; all wavefronts form the same ones)
-        const float2 x = i0 + lane < splits ? ml[i0 + lane] : make_float2(-INFINITY, 0.0f);
+        const float2 x = i0 + lane < splits ? ml[(int64_t)(i0 + lane) * a.heads] : make_float2(-INFINITY, 0.0f);
         const float f = __builtin_amdgcn_exp2f(x.x - ref);
         total += f * x.y;
         __syncthreads();
@@ -154,7 +169,7 @@ __global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a
         __syncthreads();
         const int most = splits - i0 < 64 ? splits - i0 : 64;
 #pragma unroll 8
-        for (int i = part; i < most; i += PARTS) sum = fmaf(factor[i], o[(int64_t)(i0 + i) * D + d], sum);
+        for (int i = part; i < most; i += PARTS) sum = fmaf(factor[i], o[(int64_t)(i0 + i) * a.heads * D + d], sum);
     }
     total = wave_sum(total);
     so[part][d] = sum;
@@ -165,27 +180,20 @@ __global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a
     out[d] = from_float<T>(sum / total);
 }
 
-struct plan { int nt, gw, split_len, n_splits, lds; };
+struct plan { cut t; int gw, lds; };
 
-// Keys per step, heads per workgroup, keys per split.
+// Keys per step, heads per workgroup, items.
 int plan_of(const mta_cache *c, int64_t longest, int R, int S, int window, plan &p)
 {
-    const int size = dtype_size(c->dtype), share = c->heads / c->kv_heads, wide = c->head_dim * size > 256 ? 2 : 4;
+    const int size = dtype_size(c->dtype), share = c->heads / c->kv_heads;
     const int64_t span = span_of(longest, window, 1);
-    for (int gw = 4; gw >= 1; gw >>= 1) {
-        if (share % gw) continue;
-        for (int nt = wide;; nt = 1) {
-            const int lds = raw_layout_of(gw * R, R, S, gw, c->head_dim, size, nt, true).total;
-            const int64_t steps = (span + 64 * nt - 1) / (64 * nt), groups = (int64_t)c->slots * (c->heads / gw);
-            // (long steps only where they still make enough workgroups)
-            if (lds <= (nt == 1 ? 160 << 10 : 80 << 10) && (nt == 1 || steps * groups >= 512)) {
-                const int64_t per = (steps * groups + 1023) / 1024;
-                p.nt = nt, p.gw = gw, p.lds = lds, p.split_len = (int)(per < steps ? per : steps) * 64 * nt;
-                p.n_splits = (int)((span + p.split_len - 1) / p.split_len);
-                return MTA_OK;
-            }
-            if (nt == 1) break;
-        }
+    for (p.gw = 4; p.gw >= 1; p.gw >>= 1) {
+        if (share % p.gw) continue;
+        int most = most_tiles(c->head_dim * size);
+        while (most > 1 && raw_layout_of(p.gw * R, R, S, p.gw, c->head_dim, size, most, true).total > 80 << 10) most >>= 1;
+        p.t = cut_of(span, c->slots, c->heads / p.gw, most);
+        p.lds = raw_layout_of(p.gw * R, R, S, p.gw, c->head_dim, size, p.t.nt, true).total;
+        if (p.lds <= (p.gw == 1 ? 160 << 10 : 80 << 10)) return too_many(p.t, c->heads / p.gw) ? MTA_ERR_SHAPE : MTA_OK;
     }
     return MTA_ERR_KERNEL_SIZE;
 }
@@ -194,18 +202,22 @@ template <typename T, int D, int NT, int GW> int launch(const decode_args &a, co
 {
     auto kern = conv_attn_decode_kernel<T, D, NT, GW>;
     if (const int e = allow_lds(kern, p.lds)) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)p.n_splits, (unsigned)(a.heads / GW), (unsigned)a.slots), dim3(256), p.lds, st, a);
-    if (p.n_splits > 1) hipLaunchKernelGGL((conv_attn_join_kernel<T, D>), dim3((unsigned)a.heads, (unsigned)a.slots), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.items * (a.heads / GW))), dim3(256), p.lds, st, a);
+    if (p.t.joined) hipLaunchKernelGGL((conv_attn_join_kernel<T, D>), dim3((unsigned)a.heads, (unsigned)a.slots), dim3(256), 0, st, a, 64 * NT);
     return launch_status();
 }
-template <typename T, int D, int NT> int launch_heads(const decode_args &a, const plan &p, hipStream_t st)
+template <typename T, int D, int GW> int launch_steps(const decode_args &a, const plan &p, hipStream_t st)
 {
-    return p.gw == 4 ? launch<T, D, NT, 4>(a, p, st) : p.gw == 2 ? launch<T, D, NT, 2>(a, p, st) : launch<T, D, NT, 1>(a, p, st);
+    constexpr int MOST = most_tiles(D * (int)sizeof(T));
+    if constexpr (MOST >= 4)
+        if (p.t.nt == 4) return launch<T, D, 4, GW>(a, p, st);
+    if constexpr (MOST >= 2)
+        if (p.t.nt == 2) return launch<T, D, 2, GW>(a, p, st);
+    return launch<T, D, 1, GW>(a, p, st);
 }
-template <typename T, int D> int launch_steps(const decode_args &a, const plan &p, hipStream_t st)
+template <typename T, int D> int launch_heads(const decode_args &a, const plan &p, hipStream_t st)
 {
-    constexpr int WIDE = D * (int)sizeof(T) > 256 ? 2 : 4;
-    return p.nt == 1 ? launch_heads<T, D, 1>(a, p, st) : launch_heads<T, D, WIDE>(a, p, st);
+    return p.gw == 4 ? launch_steps<T, D, 4>(a, p, st) : p.gw == 2 ? launch_steps<T, D, 2>(a, p, st) : launch_steps<T, D, 1>(a, p, st);
 }
 
 int check_args(const mta_cache *c, int64_t longest, int R, int S, int window)
@@ -226,7 +238,7 @@ extern "C" int64_t mta_conv_attn_decode_workspace(const mta_cache *c, int64_t lo
     if (const int e = check_args(c, longest, R, S, window)) return e;
     plan p;
     if (const int e = plan_of(c, longest, R, S, window, p)) return e;
-    return p.n_splits == 1 ? 0 : (stats_offset(c->slots, c->heads, p.n_splits, c->head_dim) + 2 * (int64_t)c->slots * c->heads * p.n_splits) * 4;
+    return !p.t.joined ? 0 : (stats_offset(p.t.items, c->heads, c->head_dim) + 2 * (int64_t)p.t.items * c->heads) * 4;
 }
 
 extern "C" int mta_conv_attn_decode(const mta_cache *c, const void *w, void *o, void *workspace, int64_t workspace_bytes, int64_t longest, int R, int S,
@@ -241,7 +253,7 @@ extern "C" int mta_conv_attn_decode(const mta_cache *c, const void *w, void *o, 
     const int64_t need = mta_conv_attn_decode_workspace(c, longest, R, S, window);
     if (need > 0 && (!workspace || workspace_bytes < need)) return MTA_ERR_WORKSPACE;
     decode_args a = args_of(c, w, R, S, 1, window, longest, scale, w_dtype);
-    a.o = o, a.ws = (float *)workspace, a.split_len = p.split_len, a.n_splits = p.n_splits, a.gw = p.gw;
+    a.o = o, a.ws = (float *)workspace, a.target = p.t.target, a.least = p.t.least, a.items = p.t.items, a.gw = p.gw;
     const hipStream_t st = (hipStream_t)stream;
-    MTA_DISPATCH_IO(c->dtype, return c->head_dim == 64 ? launch_steps<io_t, 64>(a, p, st) : launch_steps<io_t, 128>(a, p, st));
+    MTA_DISPATCH_IO(c->dtype, return c->head_dim == 64 ? launch_heads<io_t, 64>(a, p, st) : launch_heads<io_t, 128>(a, p, st));
 }

@@ -19,7 +19,7 @@ struct mta_args {
     int pre_group, post_group;  // heads that mix (1: the identity, no weight)
     int R2, S2, span;           // span: keys that a row of the workspace has room for
     int chunk, chunks;          // keys per workgroup of the mixing kernel
-    int v_len, v_splits;        // keys per split of the values kernel
+    int v_target, v_least, v_items, v_ch;   // the values kernel's items
     float *s1, *s2, *p1, *part;
     float *stats;               // (slot, head, row, chunk): reference, sum of exponentials
 };
@@ -40,44 +40,51 @@ __global__ __launch_bounds__(256) void decode_scores_kernel(const mta_args m)
 {
     extern __shared__ __align__(16) unsigned char smem[];
     const decode_args &a = m.d;
-    const int b = blockIdx.z, h0 = blockIdx.y * a.gw, split = blockIdx.x;
-    const slot_step s = step_of(m, b);
-    if (s.n <= 0) return;
-    const int beg = s.base + split * a.split_len;
-    if (beg >= s.n) return;
-    const int end = beg + a.split_len < s.n ? beg + a.split_len : s.n;
+    constexpr int CH = 64 * NT, SUBS = 16 / NT;
+    const int lane = threadIdx.x & 63, groups = a.heads / a.gw, index = blockIdx.x / groups, h0 = (blockIdx.x - index * groups) * a.gw;
+    const shares sh(a, m.R2 - 1, CH, false, lane);
+    const work_item it = item_of(sh, index, lane);
+    if (it.slot < 0 || it.s.n <= 0) return;
+    const slot_step s = it.s;
+    const int b = it.slot, beg = s.base + (index - it.first) * sh.per * CH, end = beg + sh.per * CH < s.n ? beg + sh.per * CH : s.n;
+    page_map pages;
+    pages.load(a, b, beg - halo_left(a.S), lane);
 
-    constexpr int CH = 64 * NT, QUADS = 4 * NT, SUBS = 64 / QUADS;
-    const int rows = a.gw * a.W, left = (a.S - 1) / 2, reach = end + a.S - 1 - left;
+    using lanes = score_lanes<NT, 1>;
+    const int rows = a.gw * a.W, right = a.S - 1 - (a.S - 1) / 2;
     const raw_layout l = raw_layout_of(rows, a.R, a.S, a.gw, D, (int)sizeof(T), NT, false);
-    raw_scores<T, D, NT> sc(a, smem, l, rows, b, h0 / a.share, s.n, reach < s.n ? reach : s.n);
-    const int lane = sc.lane, wave = sc.wave, quad = lane % QUADS, sub = lane / QUADS;
+    raw_scores<T, D, NT> sc(a, smem, l, pages, rows, h0 / a.share, s.n, end + right < s.n ? end + right : s.n);
+    const int wave = sc.wave;
+    const lanes me(lane);
     const float *const weights = reinterpret_cast<const float *>(smem + l.weights);
     const int sp = (a.S + 3) & ~3;
 
+    typename raw_scores<T, D, NT>::start st;
+    sc.begin(st, beg, b, h0);
     sc.load_step(beg);
-    sc.stage(smem, l, b, h0);
-    __syncthreads();
-    sc.halo(beg);
+    sc.finish(st, beg, b, h0, smem, l);
     int step = 0;
     for (int kb = beg; kb < end; kb += CH, ++step) {
         sc.score_step(kb, step);
-        if (kb + CH < end) sc.load_step(kb + CH);
+        if (kb + CH < end) {   // (nothing else is under way here)
+            sc.pages.reach(a, b, kb + CH, kb + 2 * CH + sc.hr < sc.limit ? kb + 2 * CH + sc.hr : sc.limit, lane);
+            sc.load_step(kb + CH);
+        }
         __syncthreads();
-        const int local = wave * 16 * NT + 4 * quad, key = kb + local;
+        const int local = wave * 16 * NT + 4 * me.quad, key = kb + local;
         float *const out = m.s1 + ((int64_t)b * a.heads + h0) * m.R2 * m.span + (key - s.base);
         for (int g = 0; g < a.gw; ++g) {
             const float *const w = weights + g * a.R * sp;
             if constexpr (ONE) {
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 with_taps(a.S, [&](auto count) {
-                    for (int r = sub; r < a.R; r += SUBS)
-                        taps4<decltype(count)::value>(part, sc.window(step, g * a.W + r, local), w + r * sp, a.S);
+                    for (int r = me.part; r < a.R; r += SUBS)
+                        taps4<decltype(count)::value>(c, sc.window(step, g * a.W + r, local), w + r * sp, a.S);
                 });
-                const float c = deal4<NT>(part);
-                if (lane % 16 < QUADS && key + lane / 16 < end) out[(int64_t)g * m.span + lane / 16] = c * a.scale;
+                me.deal(c);
+                if (me.owner && key + lane / 16 < end) out[(int64_t)g * m.span + lane / 16] = c[0] * a.scale;
             } else {
-                for (int j0 = sub * JB; j0 < m.R2; j0 += SUBS * JB) {
+                for (int j0 = me.part * JB; j0 < m.R2; j0 += SUBS * JB) {
                     float c[JB][4];
 #pragma unroll
                     for (int u = 0; u < JB; ++u) c[u][0] = c[u][1] = c[u][2] = c[u][3] = 0.0f;
@@ -101,19 +108,28 @@ __global__ __launch_bounds__(256) void decode_scores_kernel(const mta_args m)
 }
 
 // ---- mixing ahead of the softmax, and the statistics of the rows ----
-// A wavefront takes blocks of four heads of a group, a lane a key of each 64; (reference, sum) run along per lane and meet at the end.
+// A wavefront takes blocks of four heads of a group, a lane four keys of each 256 (16 bytes per load); (reference, sum) run along per lane and meet
+// at the end.
 __global__ __launch_bounds__(256) void decode_mix_kernel(const mta_args m)
 {
     extern __shared__ __align__(16) float lds[];
-    const int b = blockIdx.z, j = blockIdx.y, chunk = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int b = blockIdx.z, j = blockIdx.x, chunk = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const slot_step s = step_of(m, b);
     if (s.n <= 0) return;
     const int k0 = s.base + chunk * m.chunk, pos = row_pos(m, s.n, j), H = m.d.heads, grp = m.pre_group;
     if (k0 >= s.n) return;
     const int end = k0 + m.chunk < s.n ? k0 + m.chunk : s.n, per = (grp + 3) / 4, blocks = H / grp * per;
+    const int64_t head = (int64_t)m.R2 * m.span, row0 = (int64_t)b * H * head + (int64_t)j * m.span - s.base;
     f32x4 *const w = reinterpret_cast<f32x4 *>(lds) + wave * grp;
     for (int blk = wave; blk < blocks; blk += 4) {
         const int g0 = blk / per * grp, o0 = g0 + (blk % per) * 4, cnt = g0 + grp - o0 < 4 ? g0 + grp - o0 : 4;
+        constexpr int AHEAD = 8;
+        f32x4 first[AHEAD];   // (the first keys of the first heads: under way before the weights are)
+        {
+            const float *x = m.s1 + row0 + g0 * head + (k0 + 4 * lane < end ? k0 + 4 * lane : k0);
+#pragma unroll
+            for (int g = 0; g < AHEAD; ++g) first[g] = *reinterpret_cast<const f32x4 *>(x + (g < grp ? g : 0) * head);
+        }
         if (m.w_pre) {
             wave_sync();
             for (int x = lane; x < grp * 4; x += 64)
@@ -123,43 +139,59 @@ __global__ __launch_bounds__(256) void decode_mix_kernel(const mta_args m)
         float top[4], sum[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) top[u] = -INFINITY, sum[u] = 0.0f;
-        for (int kk = k0; kk < end; kk += 64) {
-            const int key = kk + lane;
-            const bool in = key < end, seen = in && sees(m, pos, key);
-            f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
-            const float *x = m.s1 + (((int64_t)b * H + g0) * m.R2 + j) * m.span + (in ? key - s.base : 0);
-            const int64_t head = (int64_t)m.R2 * m.span;
+        for (int key = k0 + 4 * lane; key < end; key += 256) {   // (a row has room for whole vectors)
+            f32x4 c[4];
+            const float *x = m.s1 + row0 + g0 * head + key;
+            const bool begun = key < k0 + 256;
             if (m.w_pre) {
-#pragma unroll 4
-                for (int g = 0; g < grp; ++g) {
-                    const float v = x[g * head];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) c[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                auto add = [&](int g, const f32x4 &v) {
                     const f32x4 wg = w[g];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) c[u] = fmaf(wg[u], v, c[u]);
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[u][e] = fmaf(wg[u], v[e], c[u][e]);
+                };
+                if (begun) {
+#pragma unroll
+                    for (int g = 0; g < AHEAD; ++g)
+                        if (g < grp) add(g, first[g]);
                 }
+#pragma unroll 8
+                for (int g = begun ? AHEAD : 0; g < grp; ++g) add(g, *reinterpret_cast<const f32x4 *>(x + g * head));
             } else {
-                c[0] = x[0];   // (groups of one head)
+                c[0] = begun ? first[0] : *reinterpret_cast<const f32x4 *>(x);   // (groups of one head)
+                c[1] = c[2] = c[3] = c[0];
             }
+            bool seen[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) seen[e] = key + e < end && sees(m, pos, key + e);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if (u >= cnt) break;
-                if (m.w_pre && in) m.s2[(((int64_t)b * H + o0 + u) * m.R2 + j) * m.span + (key - s.base)] = c[u];
-                if (seen) {
-                    const float e = c[u] * LOG2E, t = fmaxf(top[u], e), ref = t == -INFINITY ? 0.0f : t;
-                    sum[u] = sum[u] * __builtin_amdgcn_exp2f(top[u] - ref) + __builtin_amdgcn_exp2f(e - ref);
-                    top[u] = t;
+                if (m.w_pre && u < cnt) *reinterpret_cast<f32x4 *>(m.s2 + row0 + (o0 + u) * head + key) = c[u];
+                float t = top[u];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    c[u][e] = seen[e] ? c[u][e] * LOG2E : -INFINITY;
+                    t = fmaxf(t, c[u][e]);
                 }
+                const float ref = t == -INFINITY ? 0.0f : t;
+                sum[u] *= __builtin_amdgcn_exp2f(top[u] - ref);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[u] += seen[e] ? __builtin_amdgcn_exp2f(c[u][e] - ref) : 0.0f;
+                top[u] = t;
             }
         }
+        // (all four heads, whether they are there or not: their reductions run beside one another)
+        float t[4], l[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (u >= cnt) break;
-            const float t = wave_max(top[u]), ref = t == -INFINITY ? 0.0f : t;
-            const float l = wave_sum(sum[u] * __builtin_amdgcn_exp2f(top[u] - ref));
-            if (lane == 0) {
-                float *st = m.stats + ((((int64_t)b * H + o0 + u) * m.R2 + j) * m.chunks + chunk) * 2;
-                st[0] = t, st[1] = l;
-            }
+        for (int u = 0; u < 4; ++u) t[u] = wave_max(top[u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l[u] = wave_sum(sum[u] * __builtin_amdgcn_exp2f(top[u] - (t[u] == -INFINITY ? 0.0f : t[u])));
+        if (lane < cnt) {
+            const float tl = lane == 0 ? t[0] : lane == 1 ? t[1] : lane == 2 ? t[2] : t[3], ll = lane == 0 ? l[0] : lane == 1 ? l[1] : lane == 2 ? l[2] : l[3];
+            *reinterpret_cast<float2 *>(m.stats + ((((int64_t)b * H + o0 + lane) * m.R2 + j) * m.chunks + chunk) * 2) = make_float2(tl, ll);
         }
     }
 }
@@ -184,41 +216,67 @@ template <int PARTS> __device__ __forceinline__ float2 row_statistics(const floa
 }
 
 // ---- the conv behind the softmax: probabilities of R2 rows of a head, one row out ----
+// A wavefront takes 256 keys of one head, four to a lane: those that its taps reach included, so that a row is one load.  Its probabilities lie in
+// its own part of LDS.
+__host__ __device__ __forceinline__ int post_left(int S2) { return ((S2 - 1) / 2 + 3) & ~3; }
+__host__ __device__ __forceinline__ int post_keys(int S2) { return 256 - post_left(S2) - ((S2 - 1 - (S2 - 1) / 2 + 3) & ~3); }   // results
+constexpr int POST_STRIDE = 256 + 12;
+__host__ __device__ __forceinline__ int post_floats(int R2, int S2) { return 2 * up16(R2) + R2 * (((S2 + 3) & ~3) + POST_STRIDE); }
+
 __global__ __launch_bounds__(256) void decode_post_kernel(const mta_args m)
 {
     extern __shared__ __align__(16) float lds[];
-    const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    const int b = blockIdx.z, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), H = m.d.heads;
+    const int h = blockIdx.x * (blockDim.x >> 6) + wave;
     const slot_step s = step_of(m, b);
-    if (s.n <= 0) return;
-    const int k0 = s.base + blockIdx.x * 256;
-    if (k0 >= s.n) return;
-    const int left = (m.S2 - 1) / 2, cols = 256 + m.S2 - 1, taps = m.R2 * m.S2, H = m.d.heads;
-    float2 *const stat = reinterpret_cast<float2 *>(lds);
-    float *const w = lds + 2 * m.R2, *const p = w + taps;
+    const int k0 = s.base + blockIdx.y * post_keys(m.S2);
+    if (h >= H || s.n <= 0 || k0 >= s.n) return;   // (nothing below waits for another wavefront)
+    const int left = (m.S2 - 1) / 2, left4 = post_left(m.S2), shift = left & 3, taps = m.R2 * m.S2, sp = (m.S2 + 3) & ~3;
+    float *const mine = lds + wave * post_floats(m.R2, m.S2), *const w = mine + 2 * up16(m.R2), *const p = w + m.R2 * sp;
+    float2 *const stat = reinterpret_cast<float2 *>(mine);
     const int64_t row0 = ((int64_t)b * H + h) * m.R2;
     const int chunks = (s.n - s.base + m.chunk - 1) / m.chunk;
-    for (int x = tid; x < m.R2 * 8; x += 256) {
-        const float2 st = row_statistics<8>(m.stats + (row0 + x / 8) * m.chunks * 2, chunks, x % 8);
-        if (x % 8 == 0) stat[x / 8] = st;
+    // (loads first: scores, which do not wait for the statistics, then weights and statistics)
+    constexpr int AHEAD = 8;
+    const int key0 = k0 - left4 + 4 * lane;
+    const float *const sc = (m.w_pre ? m.s2 : m.s1) + row0 * m.span + (key0 >= s.base && key0 < s.n ? key0 - s.base : 0);
+    f32x4 x[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) x[j] = *reinterpret_cast<const f32x4 *>(sc + (int64_t)(j < m.R2 ? j : 0) * m.span);
+#pragma unroll 4
+    for (int t = lane; t < taps; t += 64) w[t / m.S2 * sp + t % m.S2] = load_any(m.w2, m.d.w_dtype, (int64_t)h * taps + t);
+    for (int t = lane; t < m.R2 * 8; t += 64) {
+        const float2 st = row_statistics<8>(m.stats + (row0 + t / 8) * m.chunks * 2, chunks, t % 8);
+        if (t % 8 == 0) stat[t / 8] = st;
     }
-    for (int x = tid; x < taps; x += 256) w[x] = load_any(m.w2, m.d.w_dtype, (int64_t)h * taps + x);
-    __syncthreads();
-    const float *const sc = m.w_pre ? m.s2 : m.s1;
-    for (int j = 0; j < m.R2; ++j) {
-        const int pos = row_pos(m, s.n, j);
-        const float2 st = stat[j];
-        for (int c = tid; c < cols; c += 256) {
-            const int key = k0 + c - left;
-            p[j * cols + c] = key >= s.base && sees(m, pos, key) ? __builtin_amdgcn_exp2f(sc[(row0 + j) * m.span + (key - s.base)] * LOG2E - st.x) * st.y : 0.0f;
+    wave_sync();
+    for (int j0 = 0; j0 < m.R2; j0 += AHEAD) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (j0 + j >= m.R2) break;
+            const int pos = row_pos(m, s.n, j0 + j);
+            const float2 st = stat[j0 + j];
+            float *const to = p + (j0 + j) * POST_STRIDE + shift + 4 * lane;   // (the taps of a lane's keys begin on 16 bytes)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                to[e] = key0 + e >= s.base && sees(m, pos, key0 + e) ? __builtin_amdgcn_exp2f(x[j][e] * LOG2E - st.x) * st.y : 0.0f;
+        }
+        if (j0 + AHEAD < m.R2) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) x[j] = *reinterpret_cast<const f32x4 *>(sc + (int64_t)(j0 + AHEAD + j < m.R2 ? j0 + AHEAD + j : 0) * m.span);
         }
     }
-    __syncthreads();
-    const int key = k0 + tid;
-    if (key >= s.n) return;
-    float c = 0.0f;
-    for (int j = 0; j < m.R2; ++j)
-        for (int t = 0; t < m.S2; ++t) c = fmaf(w[j * m.S2 + t], p[j * cols + tid + t], c);
-    m.p1[((int64_t)b * H + h) * m.span + (key - s.base)] = key >= s.lo ? c : 0.0f;
+    wave_sync();
+    const int key = k0 + 4 * lane;
+    if (4 * lane >= post_keys(m.S2) || key >= s.n) return;
+    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float *const from = p + shift + 4 * lane + left4 - left;
+    with_taps(m.S2, [&](auto count) {
+        for (int j = 0; j < m.R2; ++j) taps4<decltype(count)::value>(c, from + j * POST_STRIDE, w + j * sp, m.S2);
+    });
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = key + e >= s.lo ? c[e] : 0.0f;
+    *reinterpret_cast<f32x4 *>(m.p1 + ((int64_t)b * H + h) * m.span + (key - s.base)) = f32x4{c[0], c[1], c[2], c[3]};
 }
 
 // ---- mixing behind the softmax and P V: V once ----
@@ -227,25 +285,49 @@ template <typename T, int D, int NT, int GW, bool POST>
 __global__ __launch_bounds__(256) void decode_values_kernel(const mta_args m)
 {
     extern __shared__ __align__(16) float lds[];
-    const decode_args &a = m.d;
-    const int b = blockIdx.z, h0 = blockIdx.y * GW, split = blockIdx.x, tid = threadIdx.x;
-    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), H = a.heads, grp = m.post_group;
+    decode_args a = m.d;
+    a.target = m.v_target, a.least = m.v_least, a.items = m.v_items;
+    constexpr int CH = 64 * NT;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), H = a.heads, grp = m.post_group;
+    const int groups = H / GW, index = blockIdx.x / groups, h0 = (blockIdx.x - index * groups) * GW;
+    const shares sh(a, m.R2 - 1, CH, true, lane);
+    const work_item it = item_of(sh, index, lane);
+    if (it.slot < 0) return;
+    const slot_step s = it.s;
+    const int b = it.slot;
     T *const out = (T *)a.o + ((int64_t)b * H + h0) * D;
-    const slot_step s = step_of(m, b);
     if (s.n <= 0) {
-        if (m.v_splits == 1)
-            for (int x = tid; x < GW * D; x += 256) out[x] = from_float<T>(s.n < 0 ? __builtin_nanf("") : 0.0f);
+        for (int x = tid; x < GW * D; x += 256) out[x] = from_float<T>(s.n < 0 ? __builtin_nanf("") : 0.0f);
         return;
     }
-    const int first_key = s.lo & ~15, beg = first_key + split * m.v_len;
-    if (beg >= s.n) return;
-    const int end = beg + m.v_len < s.n ? beg + m.v_len : s.n;
-
-    constexpr int CH = 64 * NT, SUBS = 4 / NT;
-    const int sub = lane / (16 * NT), mine = lane % (16 * NT);
+    const int beg = (s.lo & ~15) + (index - it.first) * sh.per * CH, end = beg + sh.per * CH < s.n ? beg + sh.per * CH : s.n;
+    page_map pages;
+    pages.load(a, b, beg, lane);
+    using lanes = score_lanes<NT, GW>;
+    const lanes me(lane);
     float2 *const coef = reinterpret_cast<float2 *>(lds);               // [GW][grp]: reference, weight / sum
-    float *const probs = lds + 2 * GW * grp + wave * GW * 16 * NT;
-    float *const res = lds + 2 * GW * grp + DECODE_WAVES * GW * 16 * NT;
+    float *const probs = lds + 2 * up16(GW * grp) + wave * GW * 16 * NT;
+    float *const res = lds + 2 * up16(GW * grp) + DECODE_WAVES * GW * 16 * NT;
+    const int kvh = h0 / a.share;
+
+    // what a lane mixes: its quad's keys of the heads part, part + RG, .. of its head's group
+    const float *const src = (POST ? m.p1 : m.w_pre ? m.s2 : m.s1) + ((int64_t)b * H + (h0 + me.head) / grp * grp) * m.span - s.base;   // (one row per head)
+    const float2 *const mix = coef + me.head * grp;
+    constexpr int AHEAD = 2;    // loads of the next step that are under way while this one is multiplied
+    f32x4 next[AHEAD];
+    value_rows<T, D, NT, GW> val;
+    auto fetch = [&](int i, int first) {
+        const int key = first + 4 * me.quad;   // (whole vectors: where the quad begins behind the last key, of the row's first ones)
+        return *reinterpret_cast<const f32x4 *>(src + (int64_t)(i < grp ? i : 0) * m.span + (key < s.n ? key : s.base));
+    };
+    auto ahead = [&](int kb) {
+        const int first = kb + wave * 16 * NT;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) next[u] = fetch(me.part + u * lanes::RG, first);
+        val.load(a, pages, kvh, first, s.lo, end, lane);
+    };
+    ahead(beg);
+    val.clear();
     for (int x = tid; x < GW * grp * 8; x += 256) {
         const int g = x / 8 / grp, i = x / 8 - g * grp, from = (h0 + g) / grp * grp + i;
         float2 st = make_float2(0.0f, 1.0f);
@@ -256,47 +338,47 @@ __global__ __launch_bounds__(256) void decode_values_kernel(const mta_args m)
         }
     }
     __syncthreads();
-    const int *const entries = a.table + (int64_t)b * a.max_pages;
-    const int kvh = h0 / a.share;
-    auto tile = [&](int key0) -> const char * {
-        const int entry = entries[key0 >> a.page_shift];
-        if ((unsigned)entry >= (uint64_t)a.n_pages) return nullptr;
-        return a.v + ((((int64_t)entry * a.kv_heads + kvh) << a.page_shift) + (key0 & ((1 << a.page_shift) - 1))) * (D * (int)sizeof(T));
-    };
-    const float *const src = POST ? m.p1 : m.w_pre ? m.s2 : m.s1;       // (one row per head either way)
-    value_rows<T, D, NT, GW> val;
-    val.clear();
-    for (int kb = beg; kb < end; kb += CH) {
-        const int first = kb + wave * 16 * NT, key = first + mine;
-        val.load(first, s.lo, end, lane, tile);
-        const bool seen = key >= s.lo && key < end;
-        const int at = seen ? key - s.base : 0;
+    auto advance = [&](int kb, auto more) {
+        const int first = kb + wave * 16 * NT;
+        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto add = [&](int i, const f32x4 &v) {
+            if (i < grp) {
+                const float2 f = mix[i];
 #pragma unroll
-        for (int g = 0; g < GW; ++g) {
-            const float *x = src + ((int64_t)b * H + (h0 + g) / grp * grp) * m.span + at;
-            float p = 0.0f;
-#pragma unroll 4
-            for (int i = sub; i < grp; i += SUBS) {
-                const float2 c = coef[g * grp + i];
-                const float v = x[(int64_t)i * m.span];
-                p = fmaf(c.y, POST ? v : __builtin_amdgcn_exp2f(v * LOG2E - c.x), p);
+                for (int e = 0; e < 4; ++e) c[e] = fmaf(f.y, POST ? v[e] : __builtin_amdgcn_exp2f(v[e] * LOG2E - f.x), c[e]);
             }
-            if constexpr (SUBS >= 2) p = across32(p, [](float u, float v) { return u + v; });
-            if constexpr (SUBS == 4) p = across16(p, [](float u, float v) { return u + v; });
-            if (sub == 0) probs[g * 16 * NT + mine] = seen ? p : 0.0f;
+        };
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) add(me.part + u * lanes::RG, next[u]);
+#pragma unroll 4
+        for (int i = me.part + AHEAD * lanes::RG; i < grp; i += lanes::RG) add(i, fetch(i, first));
+        me.deal(c);
+        if (me.owner) {
+#pragma unroll
+            for (int u = 0; u < lanes::VALUES; ++u) {
+                const int key = first + me.key + u;
+                probs[me.head * 16 * NT + me.key + u] = key >= s.lo && key < end ? c[u] : 0.0f;
+            }
         }
         wave_sync();
-        val.multiply(probs, lane);
+        val.multiply(probs, first, s.lo, end, lane);
+        if constexpr (more.value) {
+            pages.reach(a, b, kb + CH, kb + 2 * CH < end ? kb + 2 * CH : end, lane);
+            ahead(kb + CH);
+        }
         wave_sync();
-    }
+    };
+    int kb = beg;
+    for (; kb + CH < end; kb += CH) advance(kb, count_of<1>());
+    advance(kb, count_of<0>());
     val.store(res + wave * GW * D, lane);
     __syncthreads();
     for (int x = tid; x < GW * D; x += 256) {
         float o = 0.0f;
 #pragma unroll
         for (int w = 0; w < DECODE_WAVES; ++w) o += res[w * GW * D + x];
-        if (m.v_splits == 1) out[x] = from_float<T>(o);
-        else m.part[(((int64_t)b * H + h0 + x / D) * m.v_splits + split) * D + x % D] = o;
+        if (it.count == 1) out[x] = from_float<T>(o);
+        else m.part[((int64_t)index * H + h0) * D + x] = o;
     }
 }
 
@@ -304,18 +386,17 @@ template <typename T, int D> __global__ __launch_bounds__(256) void decode_sum_k
 {
     constexpr int PARTS = 256 / D;
     __shared__ float so[PARTS][D];
-    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D;
-    T *const out = (T *)m.d.o + ((int64_t)b * m.d.heads + h) * D;
-    const slot_step s = step_of(m, b);
-    if (s.n <= 0) {
-        if (part == 0) out[d] = from_float<T>(s.n < 0 ? __builtin_nanf("") : 0.0f);
-        return;
-    }
-    const int splits = (s.n - (s.lo & ~15) + m.v_len - 1) / m.v_len;
-    const float *o = m.part + ((int64_t)b * m.d.heads + h) * m.v_splits * D + d;
+    decode_args a = m.d;
+    a.target = m.v_target, a.least = m.v_least, a.items = m.v_items;
+    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D, lane = threadIdx.x & 63;
+    const shares sh(a, m.R2 - 1, m.v_ch, true, lane);
+    const work_item it = items_of(sh, b, lane);
+    if (it.count == 1) return;   // (that item wrote the result)
+    T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
+    const float *o = m.part + ((int64_t)it.first * a.heads + h) * D + d;
     float sum = 0.0f;
 #pragma unroll 8
-    for (int i = part; i < splits; i += PARTS) sum += o[(int64_t)i * D];
+    for (int i = part; i < it.count; i += PARTS) sum += o[(int64_t)i * a.heads * D];
     so[part][d] = sum;
     __syncthreads();
     if (part != 0) return;
@@ -326,55 +407,44 @@ template <typename T, int D> __global__ __launch_bounds__(256) void decode_sum_k
 
 // ---- host side ----
 struct plan {
-    int nt, gw, split_len, n_splits, lds;             // scores
-    int span, chunk, chunks;                          // mixing
-    int v_nt, v_gw, v_len, v_splits, v_lds, mix_lds, post_lds;
+    cut t, v;                                         // items of the scores and of the values kernel
+    int gw, lds;                                      // scores
+    int span, chunk, chunks, v_gw, v_lds, mix_lds, post_waves, post_lds;
     int64_t s1, s2, stats, p1, part, total;           // workspace, in floats
 };
 
-// keys per step (a power-of-two choice of `wide` and 1), and per split, for `groups` workgroups per split
-void cut(int64_t span, int64_t groups, int wide, int &nt, int &len, int &splits)
-{
-    nt = (span + 64 * wide - 1) / (64 * wide) * groups >= 512 ? wide : 1;
-    const int64_t steps = (span + 64 * nt - 1) / (64 * nt), per = (steps * groups + 1023) / 1024;
-    len = (int)(per < steps ? per : steps) * 64 * nt;
-    splits = (int)((span + len - 1) / len);
-}
-
 int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, bool pre, bool post_conv, int pre_group, int post_group, int window, plan &p)
 {
-    const int size = dtype_size(c->dtype), share = c->heads / c->kv_heads, wide = c->head_dim * size > 256 ? 2 : 4, D = c->head_dim, W = R + R2 - 1;
+    const int size = dtype_size(c->dtype), share = c->heads / c->kv_heads, D = c->head_dim, W = R + R2 - 1;
     const int64_t span = span_of(longest, window, R2), H = c->heads, B = c->slots;
-    p.gw = 0;
-    for (int gw = 4; gw >= 1 && !p.gw; gw >>= 1) {
-        if (share % gw) continue;
-        cut(span, B * (H / gw), wide, p.nt, p.split_len, p.n_splits);
-        p.lds = raw_layout_of(gw * W, R, S, gw, D, size, p.nt, false).total;
-        if (p.nt > 1 && p.lds > 80 << 10) {
-            cut(span, B * (H / gw), 1, p.nt, p.split_len, p.n_splits);
-            p.lds = raw_layout_of(gw * W, R, S, gw, D, size, p.nt, false).total;
-        }
-        if (p.lds <= (gw == 1 ? 160 << 10 : 80 << 10)) p.gw = gw;
+    for (p.gw = 4; p.gw >= 1; p.gw >>= 1) {
+        if (share % p.gw) continue;
+        int most = most_tiles(D * size);
+        while (most > 1 && raw_layout_of(p.gw * W, R, S, p.gw, D, size, most, false).total > 80 << 10) most >>= 1;
+        p.t = cut_of(span, B, H / p.gw, most);
+        p.lds = raw_layout_of(p.gw * W, R, S, p.gw, D, size, p.t.nt, false).total;
+        if (p.lds <= (p.gw == 1 ? 160 << 10 : 80 << 10)) break;
     }
     if (!p.gw) return MTA_ERR_KERNEL_SIZE;
-    p.span = p.split_len * p.n_splits;
+    p.span = (int)((span + 255) / 256 * 256);
     // statistics: few chunks where many rows have to be put together from them
-    const int most = R2 >= 8 ? 16 : 128 / R2;
-    const int64_t tiles = (p.span + 63) / 64;
-    p.chunk = (int)((tiles + most - 1) / most) * 64;
+    const int most = R2 >= 8 ? 16 : 128 / R2, tiles = p.span / 256;
+    p.chunk = (tiles + most - 1) / most * 256;
     p.chunks = (p.span + p.chunk - 1) / p.chunk;
     p.mix_lds = DECODE_WAVES * pre_group * 16;
-    p.post_lds = (2 * R2 + R2 * S2 + R2 * (256 + S2 - 1)) * 4;
+    for (p.post_waves = 4; p.post_waves > 1 && p.post_waves * post_floats(R2, S2) * 4 > 64 << 10;) p.post_waves >>= 1;
+    p.post_lds = p.post_waves * post_floats(R2, S2) * 4;
     p.v_gw = share % 4 == 0 ? 4 : share % 2 == 0 ? 2 : 1;
-    cut(span_of(longest, window, 1), B * (H / p.v_gw), wide, p.v_nt, p.v_len, p.v_splits);
-    p.v_lds = (2 * p.v_gw * post_group + DECODE_WAVES * p.v_gw * (16 * p.v_nt + D)) * 4;
+    p.v = cut_of(span_of(longest, window, 1), B, H / p.v_gw, most_tiles(D * size));
+    p.v_lds = (2 * up16(p.v_gw * post_group) + DECODE_WAVES * p.v_gw * (16 * p.v.nt + D)) * 4;
+    if (too_many(p.t, H / p.gw) || too_many(p.v, H / p.v_gw)) return MTA_ERR_SHAPE;
     if (p.mix_lds > 160 << 10 || p.post_lds > 160 << 10 || p.v_lds > 160 << 10) return MTA_ERR_KERNEL_SIZE;
     p.s1 = 0;
     p.s2 = p.s1 + B * H * R2 * p.span;
     p.stats = p.s2 + (pre ? B * H * R2 * p.span : 0);
     p.p1 = p.stats + 2 * B * H * R2 * p.chunks;
     p.part = p.p1 + (post_conv ? B * H * p.span : 0);
-    p.total = p.part + (p.v_splits > 1 ? B * H * p.v_splits * D : 0);
+    p.total = p.part + (p.v.joined ? (int64_t)p.v.items * H * D : 0);
     return MTA_OK;
 }
 
@@ -382,14 +452,14 @@ template <typename T, int D, int NT, int JB, bool ONE> int launch_scores(const m
 {
     auto kern = decode_scores_kernel<T, D, NT, JB, ONE>;
     if (const int e = allow_lds(kern, p.lds)) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)p.n_splits, (unsigned)(m.d.heads / p.gw), (unsigned)m.d.slots), dim3(256), p.lds, st, m);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(p.t.items * (m.d.heads / p.gw))), dim3(256), p.lds, st, m);
     return launch_status();
 }
 template <typename T, int D, int NT, int GW, bool POST> int launch_values(const mta_args &m, const plan &p, hipStream_t st)
 {
     auto kern = decode_values_kernel<T, D, NT, GW, POST>;
     if (const int e = allow_lds(kern, p.v_lds)) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)p.v_splits, (unsigned)(m.d.heads / GW), (unsigned)m.d.slots), dim3(256), p.v_lds, st, m);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(p.v.items * (m.d.heads / GW))), dim3(256), p.v_lds, st, m);
     return launch_status();
 }
 template <typename T, int D, int NT, bool POST> int launch_values_heads(const mta_args &m, const plan &p, hipStream_t st)
@@ -403,23 +473,35 @@ template <typename T, int D, int NT> int launch_scores_rows(const mta_args &m, c
     return m.R2 == 1 ? launch_scores<T, D, NT, 1, true>(m, p, st) : m.R2 <= SUBS ? launch_scores<T, D, NT, 1, false>(m, p, st)
          : m.R2 <= 2 * SUBS ? launch_scores<T, D, NT, 2, false>(m, p, st) : launch_scores<T, D, NT, 3, false>(m, p, st);
 }
+template <typename T, int D, int NT> int launch_values_conv(const mta_args &m, const plan &p, hipStream_t st)
+{
+    return m.w2 ? launch_values_heads<T, D, NT, true>(m, p, st) : launch_values_heads<T, D, NT, false>(m, p, st);
+}
 template <typename T, int D> int launch_all(const mta_args &m, const plan &p, hipStream_t st)
 {
-    constexpr int WIDE = D * (int)sizeof(T) > 256 ? 2 : 4;
+    constexpr int MOST = most_tiles(D * (int)sizeof(T));
     const unsigned slots = (unsigned)m.d.slots, heads = (unsigned)m.d.heads;
-    int e = p.nt == 1 ? launch_scores_rows<T, D, 1>(m, p, st) : launch_scores_rows<T, D, WIDE>(m, p, st);
+    int e = MTA_ERR_UNSUPPORTED;
+    if (p.t.nt == 1) e = launch_scores_rows<T, D, 1>(m, p, st);
+    if constexpr (MOST >= 2)
+        if (p.t.nt == 2) e = launch_scores_rows<T, D, 2>(m, p, st);
+    if constexpr (MOST >= 4)
+        if (p.t.nt == 4) e = launch_scores_rows<T, D, 4>(m, p, st);
     if (e) return e;
     if ((e = allow_lds(decode_mix_kernel, p.mix_lds))) return e;
-    hipLaunchKernelGGL(decode_mix_kernel, dim3((unsigned)p.chunks, (unsigned)m.R2, slots), dim3(256), p.mix_lds, st, m);
+    hipLaunchKernelGGL(decode_mix_kernel, dim3((unsigned)m.R2, (unsigned)p.chunks, slots), dim3(256), p.mix_lds, st, m);
     if (m.w2) {
         if ((e = allow_lds(decode_post_kernel, p.post_lds))) return e;
-        hipLaunchKernelGGL(decode_post_kernel, dim3((unsigned)((p.span + 255) / 256), heads, slots), dim3(256), p.post_lds, st, m);
-        e = p.v_nt == 1 ? launch_values_heads<T, D, 1, true>(m, p, st) : launch_values_heads<T, D, WIDE, true>(m, p, st);
-    } else {
-        e = p.v_nt == 1 ? launch_values_heads<T, D, 1, false>(m, p, st) : launch_values_heads<T, D, WIDE, false>(m, p, st);
+        hipLaunchKernelGGL(decode_post_kernel, dim3((heads + p.post_waves - 1) / p.post_waves, (unsigned)((p.span + post_keys(m.S2) - 1) / post_keys(m.S2)), slots), dim3(64 * p.post_waves), p.post_lds, st, m);
     }
+    e = MTA_ERR_UNSUPPORTED;
+    if (p.v.nt == 1) e = launch_values_conv<T, D, 1>(m, p, st);
+    if constexpr (MOST >= 2)
+        if (p.v.nt == 2) e = launch_values_conv<T, D, 2>(m, p, st);
+    if constexpr (MOST >= 4)
+        if (p.v.nt == 4) e = launch_values_conv<T, D, 4>(m, p, st);
     if (e) return e;
-    if (p.v_splits > 1) hipLaunchKernelGGL((decode_sum_kernel<T, D>), dim3(heads, slots), dim3(256), 0, st, m);
+    if (p.v.joined) hipLaunchKernelGGL((decode_sum_kernel<T, D>), dim3(heads, slots), dim3(256), 0, st, m);
     return launch_status();
 }
 
@@ -429,7 +511,7 @@ int check_args(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2
     if (R < 1 || S < 1 || R2 < 1 || S2 < 1 || R > MTA_MAX_FUSED_KERNEL_R || S > MTA_MAX_FUSED_KERNEL_S || R2 > MTA_MAX_FUSED_KERNEL_R
         || S2 > MTA_MAX_FUSED_KERNEL_S)
         return MTA_ERR_KERNEL_SIZE;
-    if (longest < 1 || longest > (int64_t)c->max_pages * c->page || window < 0 || c->query_rows < R + R2 - 1) return MTA_ERR_SHAPE;
+    if (longest < 1 || longest > MTA_MAX_DECODE_KEYS || longest > (int64_t)c->max_pages * c->page || window < 0 || c->query_rows < R + R2 - 1) return MTA_ERR_SHAPE;
     if (pre_group < 0 || post_group < 0 || (pre_group && c->heads % pre_group) || (post_group && c->heads % post_group)) return MTA_ERR_GROUP;
     return MTA_OK;
 }
@@ -465,9 +547,9 @@ extern "C" int mta_decode(const mta_cache *c, const void *w, const void *w_pre, 
     if (const int e = plan_of(c, longest, R, S, R2, S2, w_pre != nullptr, w2 != nullptr, m.pre_group, m.post_group, window, p)) return e;
     if (workspace_bytes < p.total * 4) return MTA_ERR_WORKSPACE;
     m.d = args_of(c, w, R, S, R2, window, longest, scale, w_dtype);
-    m.d.o = o, m.d.split_len = p.split_len, m.d.n_splits = p.n_splits, m.d.gw = p.gw;
+    m.d.o = o, m.d.target = p.t.target, m.d.least = p.t.least, m.d.items = p.t.items, m.d.gw = p.gw;
     m.w_pre = w_pre, m.w_post = w_post, m.w2 = w2, m.R2 = R2, m.S2 = S2;
-    m.span = p.span, m.chunk = p.chunk, m.chunks = p.chunks, m.v_len = p.v_len, m.v_splits = p.v_splits;
+    m.span = p.span, m.chunk = p.chunk, m.chunks = p.chunks, m.v_target = p.v.target, m.v_least = p.v.least, m.v_items = p.v.items, m.v_ch = 64 * p.v.nt;
     float *const base = (float *)workspace;
     m.s1 = base + p.s1, m.s2 = base + p.s2, m.stats = base + p.stats, m.p1 = base + p.p1, m.part = base + p.part;
     const hipStream_t st = (hipStream_t)stream;
