@@ -3,6 +3,8 @@
 
 #include "ops.hpp"
 
+#include <vector>
+
 namespace mta_host {
 
 // The cache as the C ABI takes it.  Pools, ring, table and state are used as they lie (they are written, and captured graphs keep their
@@ -129,13 +131,28 @@ inline void cache_append(const Tensor &k, const Tensor &v, const Tensor &q, cons
 
 inline void cache_copy_pages(const Tensor &k, const Tensor &v, const Tensor &pairs)
 {
-    TORCH_CHECK(k.is_cuda() && v.is_cuda(), "the pools live on ", k.device(), ": the MTA kernels only run on an AMD GPU (there is no CPU path)");
     TORCH_CHECK_VALUE(k.is_contiguous() && v.is_contiguous() && k.device() == v.device() && k.dim() >= 2 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
                       "the pools are contiguous, on one device, of one shape and dtype");
+    TORCH_CHECK_VALUE(!pairs.is_cuda() && (pairs.scalar_type() == at::kInt || pairs.scalar_type() == at::kLong) && pairs.dim() == 2 && pairs.size(1) == 2,
+                      "pairs of pages are an (n,2) int32 or int64 tensor in host memory, got ", pairs.sizes(), " ", pairs.scalar_type(), " on ", pairs.device());
+    const int64_t n = pairs.size(0), pages = k.size(0);
+    if (n == 0) return;
+    const Tensor wide = pairs.to(at::kLong).contiguous();
+    const int64_t *const p = wide.const_data_ptr<int64_t>();
+    std::vector<int32_t> list(2 * n), targets;
+    targets.reserve(n);
+    for (int64_t i = 0; i < 2 * n; ++i) {
+        TORCH_CHECK_VALUE(p[i] >= 0 && p[i] < pages, "pairs of pages name page ", p[i], ", there are 0 .. ", pages - 1);
+        list[i] = (int32_t)p[i];
+        if (i % 2 && list[i] != list[i - 1]) targets.push_back(list[i]);
+    }
+    std::sort(targets.begin(), targets.end());
+    bool clash = std::adjacent_find(targets.begin(), targets.end()) != targets.end();
+    for (int64_t i = 0; i < n && !clash; ++i) clash = list[2 * i] != list[2 * i + 1] && std::binary_search(targets.begin(), targets.end(), list[2 * i]);
+    TORCH_CHECK_VALUE(!clash, "a page is the target of two pairs, or target of one and source of another");
+    TORCH_CHECK(k.is_cuda(), "the pools live on ", k.device(), ": the MTA kernels only run on an AMD GPU (there is no CPU path)");
     const c10::OptionalDeviceGuard guard(k.device());
-    const int64_t bytes = k.size(0) ? k.numel() / k.size(0) * k.element_size() : 0;
-    if (pairs.numel() == 0) return;
-    check(mta_cache_copy_pages(out_ptr(k), out_ptr(v), k.size(0), bytes, pairs.const_data_ptr<int32_t>(), pairs.size(0), stream_of(k)), "mta_cache_copy_pages");
+    check(mta_cache_copy_pages(out_ptr(k), out_ptr(v), pages, k.numel() / pages * k.element_size(), list.data(), n, stream_of(k)), "mta_cache_copy_pages");
 }
 
 }  // namespace mta_host

@@ -7,7 +7,6 @@ from __future__ import annotations
 import math
 from typing import Optional
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -827,15 +826,5 @@ def cache_copy_pages(k: torch.Tensor, v: torch.Tensor, pairs) -> None:
     others, but no page may be the target of two pairs, nor the target of one and the source of another
     (a page copied to itself is left alone)."""
     if not isinstance(pairs, torch.Tensor):
-        pairs = torch.tensor(pairs, dtype=torch.int32).reshape(-1, 2)
-    if pairs.is_cuda or pairs.dtype not in (torch.int32, torch.int64) or pairs.dim() != 2 or pairs.size(1) != 2:
-        raise ValueError(f"pairs of pages are an (n,2) int32 or int64 tensor in host memory, got {tuple(pairs.shape)} {pairs.dtype} on {pairs.device}")
-    if pairs.numel():
-        found = pairs.numpy()
-        if found.min() < 0 or found.max() >= k.size(0):
-            raise ValueError(f"pairs of pages name pages outside 0 .. {k.size(0) - 1}")
-        moved = found[found[:, 0] != found[:, 1]]
-        uses = np.bincount(moved[:, 1], minlength=k.size(0))
-        if uses.max() > 1 or uses[moved[:, 0]].any():
-            raise ValueError("a page is the target of two pairs, or target of one and source of another")
-    _lib.host().cache_copy_pages(k, v, pairs.to(torch.int32).contiguous())
+        pairs = torch.tensor(pairs, dtype=torch.int64).reshape(-1, 2)
+    _lib.host().cache_copy_pages(k, v, pairs)
