@@ -614,16 +614,19 @@ inline int64_t span_of(int64_t longest, int window, int out_rows)
 // this way gets 5.8 to 6.1 TB/s with one or two tiles of 256-byte rows and 4.6 with four, whatever the number of workgroups.
 constexpr int most_tiles(int row_bytes) { return row_bytes >= 512 ? 1 : 512 / row_bytes; }
 // Keys per step (64 nt, nt up to `most`), and what `shares` goes by; `groups` workgroups take an item, one of them for some heads each.  Two
-// workgroups to a CU are one round, four of the shortest steps, which fewer than four of the longer ones would not fill.
+// workgroups to a CU are one round, four of the shortest steps, which fewer than four of the longer ones would not fill.  Slots of a few steps
+// stay whole where there are many of them and their results would have to be joined (conv-attention, us, shared out | whole: 16 slots x 16 heads of 256 keys 17.0 | 10.6, of
+// 512 22.2 | 14.8, of 1024 28.5 | 23.8; 1 slot of 512 10.4 | 12.7).
 struct cut { int nt, target, least, items; bool joined; };
-inline cut cut_of(int64_t span, int64_t slots, int64_t groups, int most)
+inline cut cut_of(int64_t span, int64_t slots, int64_t groups, int most, bool joins)
 {
     cut c = {};
     for (c.nt = most; c.nt >= 1; c.nt >>= 1) {
         const int64_t steps = (span + 64 * c.nt - 1) / (64 * c.nt), resident = c.nt == 1 ? 1024 : 512;
         c.target = (int)(resident / groups > 1 ? resident / groups : 1);
-        if (c.nt > 1 && steps * slots < 4 * c.target) continue;
-        c.least = c.nt == 1 ? 1 : 2;
+        const bool whole = joins && (steps <= 2 || (steps <= 8 && 32 * steps <= slots * groups));
+        if (c.nt > 1 && (whole ? span <= 32 * c.nt : steps * slots < 4 * c.target)) continue;
+        c.least = whole ? (int)steps : c.nt == 1 ? 1 : 2;
         c.joined = steps > c.least;   // (else no slot has more than one item)
         const int64_t most_items = (steps * slots > (int64_t)shares::LONG * c.target ? shares::MORE * c.target : c.target) + slots + 1;
         const int64_t all = slots * ((steps + c.least - 1) / c.least);

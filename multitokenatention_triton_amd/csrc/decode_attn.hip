@@ -191,7 +191,7 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int window, plan 
         if (share % p.gw) continue;
         int most = most_tiles(c->head_dim * size);
         while (most > 1 && raw_layout_of(p.gw * R, R, S, p.gw, c->head_dim, size, most, true).total > 80 << 10) most >>= 1;
-        p.t = cut_of(span, c->slots, c->heads / p.gw, most);
+        p.t = cut_of(span, c->slots, c->heads / p.gw, most, true);
         p.lds = raw_layout_of(p.gw * R, R, S, p.gw, c->head_dim, size, p.t.nt, true).total;
         if (p.lds <= (p.gw == 1 ? 160 << 10 : 80 << 10)) return too_many(p.t, c->heads / p.gw) ? MTA_ERR_SHAPE : MTA_OK;
     }

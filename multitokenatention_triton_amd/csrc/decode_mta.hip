@@ -421,7 +421,7 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
         if (share % p.gw) continue;
         int most = most_tiles(D * size);
         while (most > 1 && raw_layout_of(p.gw * W, R, S, p.gw, D, size, most, false).total > 80 << 10) most >>= 1;
-        p.t = cut_of(span, B, H / p.gw, most);
+        p.t = cut_of(span, B, H / p.gw, most, false);
         p.lds = raw_layout_of(p.gw * W, R, S, p.gw, D, size, p.t.nt, false).total;
         if (p.lds <= (p.gw == 1 ? 160 << 10 : 80 << 10)) break;
     }
@@ -435,7 +435,7 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
     for (p.post_waves = 4; p.post_waves > 1 && p.post_waves * post_floats(R2, S2) * 4 > 64 << 10;) p.post_waves >>= 1;
     p.post_lds = p.post_waves * post_floats(R2, S2) * 4;
     p.v_gw = share % 4 == 0 ? 4 : share % 2 == 0 ? 2 : 1;
-    p.v = cut_of(span_of(longest, window, 1), B, H / p.v_gw, most_tiles(D * size));
+    p.v = cut_of(span_of(longest, window, 1), B, H / p.v_gw, most_tiles(D * size), true);
     p.v_lds = (2 * up16(p.v_gw * post_group) + DECODE_WAVES * p.v_gw * (16 * p.v.nt + D)) * 4;
     if (too_many(p.t, H / p.gw) || too_many(p.v, H / p.v_gw)) return MTA_ERR_SHAPE;
     if (p.mix_lds > 160 << 10 || p.post_lds > 160 << 10 || p.v_lds > 160 << 10) return MTA_ERR_KERNEL_SIZE;

@@ -151,6 +151,29 @@ def test_many_workgroups(h, hkv, n_slots, length):
         check(got[b, :, 0], *seq.want(b, w, 64 ** -0.5), what=f"slot {b}")
 
 
+@pytest.mark.parametrize("h,hkv,d,page,n_slots,length,dtype", [
+    (32, 32, 64, 16, 40, 1500, torch.bfloat16),     # items of more than 64 pages
+    (8, 8, 64, 16, 70, 900, torch.float32),         # more slots than lanes, more pages than entries at a time
+    (4, 1, 128, 32, 130, 200, torch.float16),       # ... whole slots
+    (16, 4, 128, 16, 9, 2500, torch.bfloat16)])
+def test_slots_of_all_lengths(h, hkv, d, page, n_slots, length, dtype):
+    """Keys shared out over slots of very different lengths, some empty, some that sit the step out."""
+    g = torch.Generator().manual_seed(5)
+    lengths = [int(length * x) for x in torch.rand(n_slots, generator=g).pow(2).tolist()]
+    lengths[3], lengths[-1] = length, 0
+    seq = Sequences(lengths, h, hkv, d, dtype, page, 7, scatter=False)
+    w, w2 = conv_weight(h, 4, 5, dtype, seq.gen), conv_weight(h, 3, 3, dtype, seq.gen)
+    pre, post = head_weight(h, 4, dtype, seq.gen), head_weight(h, 4, dtype, seq.gen)
+    seq.feed([1 if b % 5 != 2 else 0 for b in range(n_slots)])
+    got = conv_module(w).decode(seq.cache), mta_module(w, pre, w2, post).decode(seq.cache)
+    for b in list(range(0, n_slots, 1 + n_slots // 8)) + [2, 3, n_slots - 1]:
+        if b % 5 == 2:
+            assert not got[0][b].any() and not got[1][b].any()
+            continue
+        check(got[0][b, :, 0], *seq.want(b, w, d ** -0.5), what=f"slot {b}")
+        check(got[1][b, 0], *seq.want(b, w, d ** -0.5, pre=pre, w2=w2, post=post), what=f"slot {b}")
+
+
 # ---- Multi-Token Attention ---------------------------------------------------------------------------------------------------
 MTA = [  # h, hkv, r, s, r2, s2, group (0: dense), page, lengths
     (4, 4, 3, 3, 3, 3, 0, 16, LENGTHS[0]), (8, 8, 6, 11, 0, 0, 4, 64, LENGTHS[1]), (8, 2, 6, 11, 3, 5, 2, 32, LENGTHS[1]), (16, 16, 7, 7, 7, 7, 0, 64, LENGTHS[2]),
