@@ -124,22 +124,25 @@ __device__ __forceinline__ int wave_scan(int v)
 // A slot has an item at least: somebody writes its result.  Every wavefront computes this for itself, a slot to a lane.
 struct shares {
     const decode_args &a;
-    int older, ch, per;
-    bool newest;                // the keys of the newest row only, not of all output rows
+    const int older, shift;     // output rows ahead of the newest one; log2 of the keys of a step
+    const bool newest;          // the keys of the newest row only, not of all output rows
+    int per;
+    slot_step mine;             // of the first 64 slots, one to a lane
     static constexpr int LONG = 8, SHORT = 6, MORE = 4;
 
     __device__ __forceinline__ int from(const slot_step &s) const { return newest ? s.lo & ~15 : s.base; }
-    __device__ __forceinline__ int steps(const slot_step &s) const { return s.n > 0 ? (s.n - from(s) + ch - 1) / ch : 0; }
+    __device__ __forceinline__ int steps(const slot_step &s) const { return s.n > 0 ? (s.n - from(s) + (1 << shift) - 1) >> shift : 0; }
     __device__ __forceinline__ slot_step slot(int b) const
     {
         slot_step s = {0, 0, 0};
         if (b < a.slots) s = step_of(a, b, older);
         return s;
     }
-    __device__ __forceinline__ shares(const decode_args &a_, int older_, int ch_, bool newest_, int lane) : a(a_), older(older_), ch(ch_), newest(newest_)
+    __device__ __forceinline__ shares(const decode_args &a_, int older_, int shift_, bool newest_, int lane)
+        : a(a_), older(older_), shift(shift_), newest(newest_), mine(slot(lane))
     {
-        float total = 0.0f;     // (of up to 2^40 steps; the same in every wavefront)
-        for (int b0 = 0; b0 < a.slots; b0 += 64) total += (float)steps(slot(b0 + lane));
+        float total = (float)steps(mine);     // (of up to 2^40 steps; the same in every wavefront)
+        for (int b0 = 64; b0 < a.slots; b0 += 64) total += (float)steps(slot(b0 + lane));
         total = wave_sum(total);
         per = (int)ceilf(total / (float)a.target);
         if (per > LONG) {
@@ -148,23 +151,23 @@ struct shares {
         }
         if (per < a.least) per = a.least;
     }
-    // the items of 64 slots from b0 on, one slot to a lane
     __device__ __forceinline__ int items(int b, const slot_step &s) const
     {
-        const int n = (steps(s) + per - 1) / per;
+        const int n = (int)((unsigned)(steps(s) + per - 1) / (unsigned)per);
         return b >= a.slots ? 0 : n > 1 ? n : 1;
     }
 };
-// Item `index`: its slot's step, the slot's first item and their number; slot < 0: there is no such item.
+// Item `index` (or, slot >= 0, the first one of that slot): its slot's step, the slot's first item and their number; slot < 0: there is no such item.
 struct work_item { slot_step s; int slot, first, count; };
-__device__ __forceinline__ work_item item_of(const shares &sh, int index, int lane)
+__device__ __forceinline__ work_item item_of(const shares &sh, int index, int slot, int lane)
 {
     work_item w;
     int before = 0;
+    slot_step s = sh.mine;
     for (int b0 = 0; b0 < sh.a.slots; b0 += 64) {
-        const slot_step s = sh.slot(b0 + lane);
+        if (b0 > 0) s = sh.slot(b0 + lane);
         const int n = sh.items(b0 + lane, s), upto = before + wave_scan(n);
-        const uint64_t behind = __ballot(upto > index);
+        const uint64_t behind = __ballot(slot >= 0 ? b0 + lane >= slot : upto > index);
         if (behind) {
             const int l = __builtin_ctzll(behind);
             w.slot = b0 + l;
@@ -177,25 +180,6 @@ __device__ __forceinline__ work_item item_of(const shares &sh, int index, int la
     }
     w.slot = -1;
     return w;
-}
-// ... and the items of a slot
-__device__ __forceinline__ work_item items_of(const shares &sh, int slot, int lane)
-{
-    work_item w;
-    int before = 0;
-    for (int b0 = 0;; b0 += 64) {
-        const slot_step s = sh.slot(b0 + lane);
-        const int n = sh.items(b0 + lane, s), upto = before + wave_scan(n);
-        if (slot < b0 + 64) {
-            const int l = slot - b0;
-            w.slot = slot;
-            w.count = __builtin_amdgcn_readlane(n, l);
-            w.first = __builtin_amdgcn_readlane(upto, l) - w.count;
-            w.s.n = __builtin_amdgcn_readlane(s.n, l), w.s.base = __builtin_amdgcn_readlane(s.base, l), w.s.lo = __builtin_amdgcn_readlane(s.lo, l);
-            return w;
-        }
-        before = __builtin_amdgcn_readlane(upto, 63);
-    }
 }
 
 // c += a b^T over 64 bytes of 16 rows each; a lane holds 16 bytes of row lane % 16.  (Which of the contracted elements a lane group holds is
@@ -461,6 +445,7 @@ template <int N> __device__ __forceinline__ void taps4(float (&c)[4], const floa
         }
     }
 }
+constexpr int log2_of(int x) { return x > 1 ? 1 + log2_of(x >> 1) : 0; }
 template <int N> struct count_of { static constexpr int value = N; };
 // f(count_of<S>) for the sizes with unrolled code, f(count_of<0>) for the others
 template <typename F> __device__ __forceinline__ void with_taps(int S, F f)
@@ -618,11 +603,11 @@ constexpr int most_tiles(int row_bytes) { return row_bytes >= 512 ? 1 : 512 / ro
 // stay whole where there are many of them and their results would have to be joined (conv-attention, us, shared out | whole: 16 slots x 16 heads of 256 keys 17.0 | 10.6, of
 // 512 22.2 | 14.8, of 1024 28.5 | 23.8; 1 slot of 512 10.4 | 12.7).
 struct cut { int nt, target, least, items; bool joined; };
-inline cut cut_of(int64_t span, int64_t slots, int64_t groups, int most, bool joins)
+inline cut cut_of(int64_t span, int64_t slots, int64_t groups, int most, int round, bool joins)
 {
     cut c = {};
     for (c.nt = most; c.nt >= 1; c.nt >>= 1) {
-        const int64_t steps = (span + 64 * c.nt - 1) / (64 * c.nt), resident = c.nt == 1 ? 1024 : 512;
+        const int64_t steps = (span + 64 * c.nt - 1) / (64 * c.nt), resident = c.nt == 1 ? 1024 : round;
         c.target = (int)(resident / groups > 1 ? resident / groups : 1);
         const bool whole = joins && (steps <= 2 || (steps <= 8 && 32 * steps <= slots * groups));
         if (c.nt > 1 && (whole ? span <= 32 * c.nt : steps * slots < 4 * c.target)) continue;

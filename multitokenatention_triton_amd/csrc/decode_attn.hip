@@ -17,8 +17,8 @@ __global__ __launch_bounds__(256, 2) void conv_attn_decode_kernel(const decode_a
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int CH = 64 * NT;
     const int tid = threadIdx.x, lane = tid & 63, groups = a.heads / GW, index = blockIdx.x / groups, h0 = (blockIdx.x - index * groups) * GW;
-    const shares sh(a, 0, CH, false, lane);
-    const work_item it = item_of(sh, index, lane);
+    const shares sh(a, 0, log2_of(CH), false, lane);
+    const work_item it = item_of(sh, index, -1, lane);
     if (it.slot < 0) return;
     const slot_step s = it.s;
     const int b = it.slot;
@@ -142,14 +142,14 @@ __global__ __launch_bounds__(256, 2) void conv_attn_decode_kernel(const decode_a
 
 // The items of one (slot, head), brought to one reference and added up, always in the same order.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a, int ch)
+__global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a, int shift)
 {
     constexpr int PARTS = 256 / D;
     __shared__ float so[PARTS][D], factor[64];
     const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D, lane = threadIdx.x & 63;
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
-    const shares sh(a, 0, ch, false, lane);
-    const work_item it = items_of(sh, b, lane);
+    const shares sh(a, 0, shift, false, lane);
+    const work_item it = item_of(sh, 0, b, lane);
     const int splits = it.count;
     if (splits == 1) return;   // (that item wrote the result)
     const int64_t at = (int64_t)it.first * a.heads + h;
@@ -191,7 +191,7 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int window, plan 
         if (share % p.gw) continue;
         int most = most_tiles(c->head_dim * size);
         while (most > 1 && raw_layout_of(p.gw * R, R, S, p.gw, c->head_dim, size, most, true).total > 80 << 10) most >>= 1;
-        p.t = cut_of(span, c->slots, c->heads / p.gw, most, true);
+        p.t = cut_of(span, c->slots, c->heads / p.gw, most, 512, true);
         p.lds = raw_layout_of(p.gw * R, R, S, p.gw, c->head_dim, size, p.t.nt, true).total;
         if (p.lds <= (p.gw == 1 ? 160 << 10 : 80 << 10)) return too_many(p.t, c->heads / p.gw) ? MTA_ERR_SHAPE : MTA_OK;
     }
@@ -203,7 +203,7 @@ template <typename T, int D, int NT, int GW> int launch(const decode_args &a, co
     auto kern = conv_attn_decode_kernel<T, D, NT, GW>;
     if (const int e = allow_lds(kern, p.lds)) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a.items * (a.heads / GW))), dim3(256), p.lds, st, a);
-    if (p.t.joined) hipLaunchKernelGGL((conv_attn_join_kernel<T, D>), dim3((unsigned)a.heads, (unsigned)a.slots), dim3(256), 0, st, a, 64 * NT);
+    if (p.t.joined) hipLaunchKernelGGL((conv_attn_join_kernel<T, D>), dim3((unsigned)a.heads, (unsigned)a.slots), dim3(256), 0, st, a, log2_of(64 * NT));
     return launch_status();
 }
 template <typename T, int D, int GW> int launch_steps(const decode_args &a, const plan &p, hipStream_t st)

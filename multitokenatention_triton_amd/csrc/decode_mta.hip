@@ -19,7 +19,7 @@ struct mta_args {
     int pre_group, post_group;  // heads that mix (1: the identity, no weight)
     int R2, S2, span;           // span: keys that a row of the workspace has room for
     int chunk, chunks;          // keys per workgroup of the mixing kernel
-    int v_target, v_least, v_items, v_ch;   // the values kernel's items
+    int v_target, v_least, v_items, v_shift;   // the values kernel's items
     float *s1, *s2, *p1, *part;
     float *stats;               // (slot, head, row, chunk): reference, sum of exponentials
 };
@@ -42,8 +42,8 @@ __global__ __launch_bounds__(256) void decode_scores_kernel(const mta_args m)
     const decode_args &a = m.d;
     constexpr int CH = 64 * NT, SUBS = 16 / NT;
     const int lane = threadIdx.x & 63, groups = a.heads / a.gw, index = blockIdx.x / groups, h0 = (blockIdx.x - index * groups) * a.gw;
-    const shares sh(a, m.R2 - 1, CH, false, lane);
-    const work_item it = item_of(sh, index, lane);
+    const shares sh(a, m.R2 - 1, log2_of(CH), false, lane);
+    const work_item it = item_of(sh, index, -1, lane);
     if (it.slot < 0 || it.s.n <= 0) return;
     const slot_step s = it.s;
     const int b = it.slot, beg = s.base + (index - it.first) * sh.per * CH, end = beg + sh.per * CH < s.n ? beg + sh.per * CH : s.n;
@@ -290,8 +290,8 @@ __global__ __launch_bounds__(256) void decode_values_kernel(const mta_args m)
     constexpr int CH = 64 * NT;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), H = a.heads, grp = m.post_group;
     const int groups = H / GW, index = blockIdx.x / groups, h0 = (blockIdx.x - index * groups) * GW;
-    const shares sh(a, m.R2 - 1, CH, true, lane);
-    const work_item it = item_of(sh, index, lane);
+    const shares sh(a, m.R2 - 1, log2_of(CH), true, lane);
+    const work_item it = item_of(sh, index, -1, lane);
     if (it.slot < 0) return;
     const slot_step s = it.s;
     const int b = it.slot;
@@ -389,8 +389,8 @@ template <typename T, int D> __global__ __launch_bounds__(256) void decode_sum_k
     decode_args a = m.d;
     a.target = m.v_target, a.least = m.v_least, a.items = m.v_items;
     const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D, lane = threadIdx.x & 63;
-    const shares sh(a, m.R2 - 1, m.v_ch, true, lane);
-    const work_item it = items_of(sh, b, lane);
+    const shares sh(a, m.R2 - 1, m.v_shift, true, lane);
+    const work_item it = item_of(sh, 0, b, lane);
     if (it.count == 1) return;   // (that item wrote the result)
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
     const float *o = m.part + ((int64_t)it.first * a.heads + h) * D + d;
@@ -421,7 +421,7 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
         if (share % p.gw) continue;
         int most = most_tiles(D * size);
         while (most > 1 && raw_layout_of(p.gw * W, R, S, p.gw, D, size, most, false).total > 80 << 10) most >>= 1;
-        p.t = cut_of(span, B, H / p.gw, most, false);
+        p.t = cut_of(span, B, H / p.gw, most, 1024, false);
         p.lds = raw_layout_of(p.gw * W, R, S, p.gw, D, size, p.t.nt, false).total;
         if (p.lds <= (p.gw == 1 ? 160 << 10 : 80 << 10)) break;
     }
@@ -435,7 +435,7 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
     for (p.post_waves = 4; p.post_waves > 1 && p.post_waves * post_floats(R2, S2) * 4 > 64 << 10;) p.post_waves >>= 1;
     p.post_lds = p.post_waves * post_floats(R2, S2) * 4;
     p.v_gw = share % 4 == 0 ? 4 : share % 2 == 0 ? 2 : 1;
-    p.v = cut_of(span_of(longest, window, 1), B, H / p.v_gw, most_tiles(D * size), true);
+    p.v = cut_of(span_of(longest, window, 1), B, H / p.v_gw, most_tiles(D * size), 1024, true);
     p.v_lds = (2 * up16(p.v_gw * post_group) + DECODE_WAVES * p.v_gw * (16 * p.v.nt + D)) * 4;
     if (too_many(p.t, H / p.gw) || too_many(p.v, H / p.v_gw)) return MTA_ERR_SHAPE;
     if (p.mix_lds > 160 << 10 || p.post_lds > 160 << 10 || p.v_lds > 160 << 10) return MTA_ERR_KERNEL_SIZE;
@@ -549,7 +549,7 @@ extern "C" int mta_decode(const mta_cache *c, const void *w, const void *w_pre, 
     m.d = args_of(c, w, R, S, R2, window, longest, scale, w_dtype);
     m.d.o = o, m.d.target = p.t.target, m.d.least = p.t.least, m.d.items = p.t.items, m.d.gw = p.gw;
     m.w_pre = w_pre, m.w_post = w_post, m.w2 = w2, m.R2 = R2, m.S2 = S2;
-    m.span = p.span, m.chunk = p.chunk, m.chunks = p.chunks, m.v_target = p.v.target, m.v_least = p.v.least, m.v_items = p.v.items, m.v_ch = 64 * p.v.nt;
+    m.span = p.span, m.chunk = p.chunk, m.chunks = p.chunks, m.v_target = p.v.target, m.v_least = p.v.least, m.v_items = p.v.items, m.v_shift = 6 + (p.v.nt >> 1);   // (nt: 1, 2 or 4)
     float *const base = (float *)workspace;
     m.s1 = base + p.s1, m.s2 = base + p.s2, m.stats = base + p.stats, m.p1 = base + p.p1, m.part = base + p.part;
     const hipStream_t st = (hipStream_t)stream;
