@@ -4,13 +4,16 @@
 // query row is p = n - 1.  Keys and values lie in pages (page, key head, row, element), table[b][key / page] names the page; queries in a
 // ring, position i in row i % ring.  A row i sees the keys max(0, i - window + 1) .. i; what a row does not see counts as 0 ahead of the conv.
 //
-// Work split.  A workgroup of four wavefronts takes one slot, one or more query heads of one key head, and a stretch of the keys (a "split"),
-// in steps of 64 * NT keys, 16 * NT per wavefront.  Keys are a tile of 16 consecutive rows of a page, read straight into the operand
+// Work split.  A workgroup of four wavefronts takes one slot, one or more query heads of one key head, and a stretch of the keys (an "item",
+// see shares), in steps of 64 * NT keys, 16 * NT per wavefront.  Keys are tiles of 16 consecutive rows of a page, read straight into the operand
 // fragments of 16x16 products (no key is used by two wavefronts, so LDS would only add a pass); the query rows that the conv needs, one to a
 // few tens, are the other operand, in LDS.  The conv takes what it needs of neighbouring keys from LDS, where the last columns of a step are
-// written a second time, as the first columns of the next one: a split reads (halo) keys twice only where it begins.  Three buffers of raw
+// written a second time, as the first columns of the next one: keys are read twice only where an item begins (halo).  Three buffers of raw
 // scores: one is read, the next one gets the columns to come, and the one before may still be read by a wavefront that is behind - a single
 // barrier per step.
+//
+// What bounds it: K and V are read once, 2 D elements per key and head against some 2 R D + 2 R S + 2 D operations on them, so memory - where the
+// keys are many.  Below some megabytes it is the chain from the state to the table to K to LDS to the result, 4 to 6 us a kernel.
 #pragma once
 
 #include "common.hpp"
@@ -39,7 +42,7 @@ struct decode_args {
 
 // One slot's step: n < 0: not a state of this cache, or more tokens than grid and workspace were sized for (its outputs are NaN); 0: it
 // sits this step out (zeros).  older: output rows ahead of the newest one.
-// base: where the splits begin, a multiple of 16; lo: the first key that the newest row sees.
+// base: where the items begin, a multiple of 16; lo: the first key that the newest row sees.
 struct slot_step { int n, base, lo; };
 __device__ __forceinline__ slot_step step_of(const decode_args &a, int b, int older)
 {
@@ -94,7 +97,6 @@ __device__ __forceinline__ float wave_sum(float v) { return wave_reduce(v, [](fl
 template <int STEP> __device__ __forceinline__ float lanes_sum(float v)
 {
     auto add = [](float a, float b) { return a + b; };
-    if constexpr (STEP <= 4) v = v + dpp<0x124>(v);
     if constexpr (STEP <= 8) v = v + dpp<0x128>(v);
     if constexpr (STEP <= 16) v = across16(v, add);
     if constexpr (STEP <= 32) v = across32(v, add);
@@ -115,7 +117,7 @@ __device__ __forceinline__ int wave_scan(int v)
 }
 
 // How the slots' keys are shared out over workgroups.  The host knows the longest slot at most (a captured graph: not even that), so the
-// device does it: every slot's keys in steps of `ch`, `per` steps to an item.  Items of one size, however different the lengths, and all that live
+// device does it: every slot's keys in steps, `per` of them to an item.  Items of one size, however different the lengths, and all that live
 // next to each other in the grid, which deals its workgroups over the XCDs in turn: with a grid of (split, head, slot) short slots left
 // whole XCDs idle (conv-attention, 16 slots of 1k to 8k keys 204 us, now 153; MTA, 16 slots of 512 to 4k keys 142, now 84).
 // per: `target` items are one round of workgroups that are all resident (an item costs some 5 us beside its keys - the table, queries, weights,
@@ -288,7 +290,7 @@ template <typename T, int D, int NT> struct raw_scores {
     {
     }
 
-    // A tile of keys, if it holds any that this split needs; false: it lies in no page.
+    // A tile of keys, if it holds any that this item needs; false: it lies in no page.
     __device__ __forceinline__ bool load(u32x4 (&dst)[NC], int key0, bool wanted = true) const
     {
         bool ok;
@@ -589,7 +591,7 @@ inline decode_args args_of(const mta_cache *c, const void *w, int R, int S, int 
     a.R = R, a.S = S, a.W = R + out_rows - 1, a.window = window, a.longest = (int)longest, a.scale = scale, a.w_dtype = w_dtype;
     return a;
 }
-// keys that the splits of one slot have to cover at most
+// keys that the items of one slot have to cover at most
 inline int64_t span_of(int64_t longest, int window, int out_rows)
 {
     const int64_t seen = window > 0 ? (int64_t)window + out_rows - 1 + 15 : longest;
@@ -598,10 +600,11 @@ inline int64_t span_of(int64_t longest, int window, int out_rows)
 // Keys per step and wavefront, in tiles of 16: 8 KB of K and as many of V.  More in flight is slower, not faster: a kernel that only reads pages
 // this way gets 5.8 to 6.1 TB/s with one or two tiles of 256-byte rows and 4.6 with four, whatever the number of workgroups.
 constexpr int most_tiles(int row_bytes) { return row_bytes >= 512 ? 1 : 512 / row_bytes; }
-// Keys per step (64 nt, nt up to `most`), and what `shares` goes by; `groups` workgroups take an item, one of them for some heads each.  Two
-// workgroups to a CU are one round, four of the shortest steps, which fewer than four of the longer ones would not fill.  Slots of a few steps
-// stay whole where there are many of them and their results would have to be joined (conv-attention, us, shared out | whole: 16 slots x 16 heads of 256 keys 17.0 | 10.6, of
-// 512 22.2 | 14.8, of 1024 28.5 | 23.8; 1 slot of 512 10.4 | 12.7).
+// Keys per step (64 nt, nt up to `most`), and what `shares` goes by; `groups` workgroups take an item, one of them for some heads each.  `round`
+// workgroups are one round: two to a CU with the registers for K and V, four without; of the shortest steps four.  A round of which each had
+// fewer than four steps takes shorter ones.  Slots of a few steps stay whole where there are many of them and their results would have to be
+// joined (conv-attention, us, shared out | whole: 16 slots x 16 heads of 256 keys 17.0 | 10.6, of 512 22.2 | 14.8, of 1024 28.5 | 23.8; 1 slot of
+// 512 10.4 | 12.7).
 struct cut { int nt, target, least, items; bool joined; };
 inline cut cut_of(int64_t span, int64_t slots, int64_t groups, int most, int round, bool joins)
 {

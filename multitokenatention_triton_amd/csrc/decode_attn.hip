@@ -2,7 +2,7 @@
 //   raw_i[k] = q_i . K_k where row i sees key k, else 0            (i = p - R + 1 .. p, the newest rows)
 //   s[k]     = scale * sum_{r < R, t < S} w[r][t] raw_{p - R + 1 + r}[k + t - (S-1)/2]
 //   o        = sum_k exp(s[k]) V_k / sum_k exp(s[k])               over the keys k that row p sees
-// split over the keys and joined.  Scores, statistics, probabilities and sums stay in fp32; the result is rounded once.
+// shared out over the keys and joined.  Scores, statistics, probabilities and sums stay in fp32; the result is rounded once.
 #include "decode.hpp"
 
 namespace mta {

@@ -7,7 +7,7 @@
 //   o        = sum_k p2[k] V_k
 // Heads and rows meet between the stages, so this is not one pass but four or five short kernels around the two that stream: scores (K once),
 // mixing with the rows' statistics, the second conv (none where it is the identity: a single row is left then), mixing and values (V once),
-// and the sum over the splits.  What goes between them is R2 numbers of fp32 per key and head, against 2 D of K and V.
+// and the sum over the items.  What goes between them is R2 numbers of fp32 per key and head, against 2 D of K and V.
 #include "decode.hpp"
 
 namespace mta {
@@ -438,7 +438,8 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
     p.v = cut_of(span_of(longest, window, 1), B, H / p.v_gw, most_tiles(D * size), 1024, true);
     p.v_lds = (2 * up16(p.v_gw * post_group) + DECODE_WAVES * p.v_gw * (16 * p.v.nt + D)) * 4;
     if (too_many(p.t, H / p.gw) || too_many(p.v, H / p.v_gw)) return MTA_ERR_SHAPE;
-    if (p.mix_lds > 160 << 10 || p.post_lds > 160 << 10 || p.v_lds > 160 << 10) return MTA_ERR_KERNEL_SIZE;
+    if (p.mix_lds > 160 << 10 || p.v_lds > 160 << 10) return MTA_ERR_SHAPE;
+    if (p.post_lds > 160 << 10) return MTA_ERR_KERNEL_SIZE;
     p.s1 = 0;
     p.s2 = p.s1 + B * H * R2 * p.span;
     p.stats = p.s2 + (pre ? B * H * R2 * p.span : 0);

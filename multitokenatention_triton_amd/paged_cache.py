@@ -100,7 +100,7 @@ class PagedCache:
             need = -(-n // page)
             if not 0 <= new <= n or need > table.size(1):
                 raise ValueError(f"slot {slot}: {n} tokens, {new} of them new, do not fit {table.size(1)} pages of {page}")
-            pages = [int(p) for p in table[slot, :need]]
+            pages = table[slot, :need].tolist()
             if any(not 0 <= p < k.size(0) for p in pages) or len(set(pages)) < need:
                 raise ValueError(f"slot {slot}: its pages are not {need} different ones of 0 .. {k.size(0) - 1}")
             for i, p in enumerate(pages):
@@ -110,7 +110,9 @@ class PagedCache:
         if any(o and u > 1 for o, u in zip(own, cache._uses)):
             raise ValueError("a page with new tokens, or with room for more, belongs to several slots")
         cache._free = [p for p, u in enumerate(cache._uses) if u == 0]
-        cache._upload(range(q.size(0)))
+        need = torch.tensor([len(pages) for pages in cache._pages])
+        cache._host_table.copy_(torch.where(torch.arange(table.size(1)) < need[:, None], table, -1))
+        cache._upload(everything=True)
         return cache
 
     # ------------------------------------------------------------------ bookkeeping
@@ -150,8 +152,8 @@ class PagedCache:
         if self.k.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what} is host bookkeeping and cannot be captured into a graph: call it between replays")
 
-    def _upload(self, slots=()) -> None:
-        """State, and the rows of the table of ``slots``, to the device."""
+    def _upload(self, slots=(), everything: bool = False) -> None:
+        """State, and the rows of the table of ``slots`` (``everything``: the table as it is), to the device."""
         n = self.n_slots
         self._host_state[0] = torch.tensor([have - new for have, new in zip(self._lengths, self._added)], dtype=torch.int32)
         self._host_state[1] = torch.tensor(self._added, dtype=torch.int32)
@@ -159,7 +161,7 @@ class PagedCache:
             row = self._host_table[slot]
             row.fill_(-1)
             row[:len(self._pages[slot])] = torch.tensor(self._pages[slot], dtype=torch.int32)
-        count = self._host.numel() if len(slots) else 2 * n
+        count = self._host.numel() if everything or len(slots) else 2 * n
         if self.k.is_cuda:
             # (a pinned copy of its own: the mirror may change before the stream gets there)
             with torch.cuda.device(self.k.device):

@@ -178,7 +178,7 @@ def test_slots_of_all_lengths(h, hkv, d, page, n_slots, length, dtype):
 MTA = [  # h, hkv, r, s, r2, s2, group (0: dense), page, lengths
     (4, 4, 3, 3, 3, 3, 0, 16, LENGTHS[0]), (8, 8, 6, 11, 0, 0, 4, 64, LENGTHS[1]), (8, 2, 6, 11, 3, 5, 2, 32, LENGTHS[1]), (16, 16, 7, 7, 7, 7, 0, 64, LENGTHS[2]),
     (12, 6, 5, 7, 2, 9, 6, 16, LENGTHS[1]), (4, 2, 11, 15, 11, 15, 0, 64, LENGTHS[1]), (2, 1, 1, 1, 1, 3, 0, 16, LENGTHS[2]), (4, 4, 4, 33, 5, 63, 0, 16, LENGTHS[1]),
-    (40, 8, 3, 3, 0, 0, 20, 32, LENGTHS[1]), (32, 32, 3, 3, 3, 3, 0, 32, LENGTHS[1])]
+    (40, 8, 3, 3, 0, 0, 20, 32, LENGTHS[1]), (32, 32, 3, 3, 3, 3, 0, 32, LENGTHS[1]), (2, 2, 32, 63, 32, 63, 0, 16, [200, 31])]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -357,6 +357,26 @@ def test_on_another_stream():
     stream.synchronize()
     for b in range(2):
         check(got[b, 0], *seq.want(b, w, d ** -0.5, pre=pre, w2=w2, post=post), what=f"slot {b}")
+
+
+def test_two_calls_at_once():
+    """Decodes of one cache on two streams, and of two caches, beside one another: each has its own workspace."""
+    h, d, dtype = 8, 64, torch.bfloat16
+    seqs = [Sequences([700, 90], h, h, d, dtype, 16, 7, seed=s, scatter=False) for s in (0, 1)]
+    w, w2 = conv_weight(h, 5, 7, dtype, seqs[0].gen), conv_weight(h, 3, 3, dtype, seqs[0].gen)
+    pre, post = head_weight(h, h, dtype, seqs[0].gen), head_weight(h, h, dtype, seqs[0].gen)
+    conv, full = conv_module(w), mta_module(w, pre, w2, post)
+    want = [(conv.decode(s.cache), full.decode(s.cache)) for s in seqs]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 4]):
+            s = seqs[i % 2].cache
+            got.append((conv.decode(s), full.decode(s)))
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(got):
+        assert torch.equal(a, want[i % 2][0]) and torch.equal(b, want[i % 2][1])
 
 
 def test_same_bits_every_time():
