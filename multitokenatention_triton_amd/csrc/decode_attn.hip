@@ -71,8 +71,7 @@ __global__ __launch_bounds__(256, 2) void conv_attn_decode_kernel(const decode_a
         for (int u = 0; u < lanes::VALUES; ++u) {
             const int key = first + me.key + u;
             seen[u] = key >= s.lo && key < end;
-            c[u] = seen[u] ? c[u] * scale2 : -INFINITY;
-            top = fmaxf(top, c[u]);
+            top = fmaxf(top, seen[u] ? c[u] * scale2 : -INFINITY);
         }
         top = lanes::reduce(top, [](float x, float y) { return fmaxf(x, y); });
         if (__any(top > m)) {
@@ -91,7 +90,7 @@ __global__ __launch_bounds__(256, 2) void conv_attn_decode_kernel(const decode_a
         float *const to = probs + me.head * 16 * NT + me.key;
 #pragma unroll
         for (int u = 0; u < lanes::VALUES; ++u) {
-            const float p = seen[u] ? __builtin_amdgcn_exp2f(c[u] - ref) : 0.0f;
+            const float p = seen[u] ? __builtin_amdgcn_exp2f(fmaf(c[u], scale2, -ref)) : 0.0f;   // (one rounding: the reference's own cancels)
             if (me.owner) {
                 sum += p;
                 to[u] = p;

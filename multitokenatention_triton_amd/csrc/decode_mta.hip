@@ -172,14 +172,11 @@ __global__ __launch_bounds__(256) void decode_mix_kernel(const mta_args m)
                 if (m.w_pre && u < cnt) *reinterpret_cast<f32x4 *>(m.s2 + row0 + (o0 + u) * head + key) = c[u];
                 float t = top[u];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    c[u][e] = seen[e] ? c[u][e] * LOG2E : -INFINITY;
-                    t = fmaxf(t, c[u][e]);
-                }
+                for (int e = 0; e < 4; ++e) t = fmaxf(t, seen[e] ? c[u][e] * LOG2E : -INFINITY);
                 const float ref = t == -INFINITY ? 0.0f : t;
                 sum[u] *= __builtin_amdgcn_exp2f(top[u] - ref);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[u] += seen[e] ? __builtin_amdgcn_exp2f(c[u][e] - ref) : 0.0f;
+                for (int e = 0; e < 4; ++e) sum[u] += seen[e] ? __builtin_amdgcn_exp2f(fmaf(c[u][e], LOG2E, -ref)) : 0.0f;
                 top[u] = t;
             }
         }
@@ -259,7 +256,7 @@ __global__ __launch_bounds__(256) void decode_post_kernel(const mta_args m)
             float *const to = p + (j0 + j) * POST_STRIDE + shift + 4 * lane;   // (the taps of a lane's keys begin on 16 bytes)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                to[e] = key0 + e >= s.base && sees(m, pos, key0 + e) ? __builtin_amdgcn_exp2f(x[j][e] * LOG2E - st.x) * st.y : 0.0f;
+                to[e] = key0 + e >= s.base && sees(m, pos, key0 + e) ? __builtin_amdgcn_exp2f(fmaf(x[j][e], LOG2E, -st.x)) * st.y : 0.0f;
         }
         if (j0 + AHEAD < m.R2) {
 #pragma unroll
@@ -345,7 +342,7 @@ __global__ __launch_bounds__(256) void decode_values_kernel(const mta_args m)
             if (i < grp) {
                 const float2 f = mix[i];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c[e] = fmaf(f.y, POST ? v[e] : __builtin_amdgcn_exp2f(v[e] * LOG2E - f.x), c[e]);
+                for (int e = 0; e < 4; ++e) c[e] = fmaf(f.y, POST ? v[e] : __builtin_amdgcn_exp2f(fmaf(v[e], LOG2E, -f.x)), c[e]);
             }
         };
 #pragma unroll
