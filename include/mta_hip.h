@@ -547,7 +547,7 @@ int mta_conv_attn_decode(const mta_cache *cache, const void *w, void *o, void *w
  * identity), w_pre and w_post (heads, heads) or NULL (the identity), all of dtype w_dtype; pre_group, post_group as group_size of
  * mta_headmix_fwd.  query_rows >= R + R2 - 1.  Everything else as mta_conv_attn_decode; the workspace (16-byte aligned) serves any
  * choice of NULL weights. */
-#define MTA_MAX_DECODE_KEYS (1 << 24) /* `longest` of mta_decode */
+#define MTA_MAX_DECODE_KEYS (1 << 23) /* `longest` of mta_decode (a launch has 65535 blocks of some 200 keys) */
 int64_t mta_decode_workspace(const mta_cache *cache, int64_t longest, int R, int S, int R2, int S2, int pre_group, int post_group, int window);
 int mta_decode(const mta_cache *cache, const void *w, const void *w_pre, const void *w2, const void *w_post, void *o, void *workspace,
                int64_t workspace_bytes, int64_t longest, int R, int S, int R2, int S2, int pre_group, int post_group, int window, float scale,

@@ -200,3 +200,18 @@ def test_abi_argument_codes():
     assert lib.mta_cache_copy_pages(p, p, 8, 64, pairs, 0, None) == 0
     assert lib.mta_conv_attn_decode_workspace(ctypes.byref(c), 0, 3, 3, 0) == -3 and lib.mta_conv_attn_decode_workspace(ctypes.byref(c), 64, 3, 3, 0) >= 0
     assert lib.mta_decode_workspace(ctypes.byref(c), 64, 3, 3, 3, 3, 3, 0, 0) == -5 and lib.mta_decode_workspace(ctypes.byref(c), 64, 3, 3, 3, 3, 0, 0, 0) > 0
+
+
+def test_longest_rows():
+    """Multi-Token Attention's rows go as far as its launches do, and no size on the way wraps round; single-pass attention's go further."""
+    lib = _lib.load()
+    p = 1 << 20
+    c = _lib.Cache(k=p, v=p, q=p, table=p, state=p, n_pages=1 << 20, slots=2, max_pages=1 << 20, page=1024, heads=4, kv_heads=4, head_dim=64, query_rows=64, dtype=0)
+    most = 1 << 23
+    for r2, s2 in ((1, 1), (3, 3), (32, 63)):
+        size = lib.mta_decode_workspace(ctypes.byref(c), most, 3, 3, r2, s2, 0, 0, 0)
+        assert size >= 4 * 2 * 4 * r2 * most
+        assert lib.mta_decode_workspace(ctypes.byref(c), most + 1, 3, 3, r2, s2, 0, 0, 0) == -3
+        assert lib.mta_decode(ctypes.byref(c), p, p, p, p, p, p, size, most + 1, 3, 3, r2, s2, 0, 0, 0, 0.1, 0, None) == -3
+    assert lib.mta_conv_attn_decode_workspace(ctypes.byref(c), 1 << 30, 3, 3, 0) >= 0
+    assert lib.mta_conv_attn_decode_workspace(ctypes.byref(c), (1 << 30) + 1, 3, 3, 0) == -3
