@@ -149,24 +149,24 @@ __global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
     const shares sh(a, 0, shift, false, lane);
     const work_item it = item_of(sh, 0, b, lane);
-    const int splits = it.count;
-    if (splits == 1) return;   // (that item wrote the result)
+    const int items = it.count;
+    if (items == 1) return;   // (that item wrote the result)
     const int64_t at = (int64_t)it.first * a.heads + h;
     const float *o = a.ws + at * D;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ws + stats_offset(a.items, a.heads, D)) + at;
     float top = -INFINITY;
-    for (int i = lane; i < splits; i += 64) top = fmaxf(top, ml[(int64_t)i * a.heads].x);
+    for (int i = lane; i < items; i += 64) top = fmaxf(top, ml[(int64_t)i * a.heads].x);
     top = wave_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, total = 0.0f;
-    for (int i0 = 0; i0 < splits; i0 += 64) {   // (factors of 64 splits at a time; all wavefronts form the same ones)
-        const float2 x = i0 + lane < splits ? ml[(int64_t)(i0 + lane) * a.heads] : make_float2(-INFINITY, 0.0f);
+    for (int i0 = 0; i0 < items; i0 += 64) {   // (factors of 64 items at a time; all wavefronts form the same ones)
+        const float2 x = i0 + lane < items ? ml[(int64_t)(i0 + lane) * a.heads] : make_float2(-INFINITY, 0.0f);
         const float f = __builtin_amdgcn_exp2f(x.x - ref);
         total += f * x.y;
         __syncthreads();
         if (threadIdx.x < 64) factor[lane] = f;
         __syncthreads();
-        const int most = splits - i0 < 64 ? splits - i0 : 64;
+        const int most = items - i0 < 64 ? items - i0 : 64;
 #pragma unroll 8
         for (int i = part; i < most; i += PARTS) sum = fmaf(factor[i], o[(int64_t)(i0 + i) * a.heads * D + d], sum);
     }

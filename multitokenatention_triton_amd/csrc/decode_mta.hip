@@ -5,9 +5,9 @@
 //   s2_j     = sum_g Wpre[h][g] s1_j (head g)                                         p_j = softmax over the keys that row j sees
 //   p1[k]    = sum_{r, t} w2[h][r][t] p_{P - R2 + 1 + r}[k + t - (S2-1)/2]             p2 = sum_g Wpost[h][g] p1 (head g)
 //   o        = sum_k p2[k] V_k
-// Heads and rows meet between the stages, so this is not one pass but four or five short kernels around the two that stream: scores (K once),
-// mixing with the rows' statistics, the second conv (none where it is the identity: a single row is left then), mixing and values (V once),
-// and the sum over the items.  What goes between them is R2 numbers of fp32 per key and head, against 2 D of K and V.
+// Heads and rows meet between the stages, so this is not one pass but up to five kernels, two of which stream: scores (K once), mixing with the
+// rows' statistics, the second conv (none where it is the identity: a single row is left then; one kernel with the mixing for short rows), mixing
+// and values (V once), and the sum over the items.  What goes between them is R2 numbers of fp32 per key and head, against 2 D of K and V.
 #include "decode.hpp"
 
 namespace mta {
@@ -276,6 +276,118 @@ __global__ __launch_bounds__(256) void decode_post_kernel(const mta_args m)
     *reinterpret_cast<f32x4 *>(m.p1 + ((int64_t)b * H + h) * m.span + (key - s.base)) = f32x4{c[0], c[1], c[2], c[3]};
 }
 
+// ---- mixing, softmax and the conv behind it in one kernel, for rows of up to 512 keys ----
+// A workgroup takes a block of up to four heads of a group; a wavefront an output row of all four, whole, 4 KQ keys to a lane, so that neither the
+// mixed scores nor statistics go through memory; then a wavefront 256 keys of one head for the conv, from the probabilities in LDS.  Eight
+// wavefronts, 16 above eight rows: a row more to a wavefront is a turn of loads more (rows 5 to 8 with four wavefronts: 3 us slower).
+// All kernels of a call, us, one kernel | two (3 x 3 in front; slots x heads, R2 x S2, heads that mix):
+//   250 keys  1 x 8, 3 x 3, all 16.1 | 19.3    2 x 16, 10 x 11, 4 19.1 | 26.4    32 x 16, 7 x 7, all 29.8 | 35.3
+//   500 keys  1 x 8, 3 x 3, all 18.4 | 20.6    2 x 16, 10 x 11, 4 21.9 | 27.9    32 x 16, 7 x 7, all 43.9 | 49.1
+// and with 16 keys to a lane, 1000 keys 22.3 | 21.7, 28.5 | 28.3, 78.3 | 80.5: the chain in a wavefront grows while the two kernels spread, so
+// longer rows stay with those.
+__host__ __device__ __forceinline__ int short_stride(int S2, int kq) { return post_left(S2) + 256 * kq + 12 + up16(S2); }
+__host__ __device__ __forceinline__ int short_floats(int R2, int S2, int pre_group, int kq)
+{
+    return 4 * pre_group + 4 * R2 * ((S2 + 3) & ~3) + 4 * R2 * short_stride(S2, kq);
+}
+
+template <int KQ> __global__ __launch_bounds__(1024) void decode_mix_post_kernel(const mta_args m)
+{
+    extern __shared__ __align__(16) float lds[];
+    const int tid = threadIdx.x, threads = blockDim.x, waves = threads >> 6, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = blockIdx.y, H = m.d.heads, R2 = m.R2, S2 = m.S2;
+    const slot_step s = step_of(m, b);
+    if (s.n <= 0) return;
+    const int grp = m.pre_group, per = (grp + 3) / 4, blk = blockIdx.x, g0 = blk / per * grp, o0 = g0 + blk % per * 4;
+    const int cnt = g0 + grp - o0 < 4 ? g0 + grp - o0 : 4, keys = s.n - s.base, taps = R2 * S2;
+    const int left = (S2 - 1) / 2, left4 = post_left(S2), shift = left & 3, stride = short_stride(S2, KQ), sp = (S2 + 3) & ~3;
+    // (rows: a row's key 0; the taps of every fourth key begin on 16 bytes)
+    float *const w = lds, *const w2 = w + 4 * grp, *const rows = w2 + 4 * R2 * sp + left4 + shift;
+    const int64_t head = (int64_t)R2 * m.span;
+    if (m.w_pre)
+        for (int x = tid; x < grp * 4; x += threads) w[x] = (x & 3) < cnt ? load_any(m.w_pre, m.d.w_dtype, (int64_t)(o0 + (x & 3)) * H + g0 + (x >> 2)) : 0.0f;
+#pragma unroll 2
+    for (int x = tid; x < cnt * taps; x += threads) w2[x / S2 * sp + x % S2] = load_any(m.w2, m.d.w_dtype, (int64_t)o0 * taps + x);
+    for (int r = wave; r < 4 * R2; r += waves) {   // zeros on either side of every row's keys
+        float *const row = rows + r * stride;
+        if (lane < left4 + shift) row[lane - left4 - shift] = 0.0f;
+        for (int c = keys + lane; c < stride - left4 - shift; c += 64) row[c] = 0.0f;
+    }
+    __syncthreads();
+    for (int j = wave; j < R2; j += waves) {
+        const float *const x = m.s1 + ((int64_t)b * H + g0) * head + (int64_t)j * m.span;
+        const int pos = row_pos(m, s.n, j);
+        f32x4 c[4][KQ];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < KQ; ++q) c[u][q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int g = 0; g < grp; ++g) {
+            const f32x4 wg = m.w_pre ? *reinterpret_cast<const f32x4 *>(w + 4 * g) : f32x4{1.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int q = 0; q < KQ; ++q) {
+                const int k = 256 * q + 4 * lane;
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(x + g * head + (k < keys ? k : 0));   // (a row has room for whole vectors)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[u][q][e] = fmaf(wg[u], v[e], c[u][q][e]);
+            }
+        }
+        float top[4], sum[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            top[u] = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < KQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[u] = fmaxf(top[u], sees(m, pos, s.base + 256 * q + 4 * lane + e) ? c[u][q][e] * LOG2E : -INFINITY);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) top[u] = wave_max(top[u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float ref = top[u] == -INFINITY ? 0.0f : top[u];
+            sum[u] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < KQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    c[u][q][e] = sees(m, pos, s.base + 256 * q + 4 * lane + e) ? __builtin_amdgcn_exp2f(fmaf(c[u][q][e], LOG2E, -ref)) : 0.0f;
+                    sum[u] += c[u][q][e];
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[u] = wave_sum(sum[u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (u >= cnt) break;
+            const float f = pos >= 0 ? 1.0f / sum[u] : 0.0f;   // (a row ahead of the first token sees nothing)
+            float *const to = rows + (u * R2 + j) * stride;
+#pragma unroll
+            for (int q = 0; q < KQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int k = 256 * q + 4 * lane + e;
+                    if (k < keys) to[k] = c[u][q][e] * f;
+                }
+        }
+    }
+    __syncthreads();
+    const int u = wave & 3;   // (eight or 16 wavefronts)
+    if (u >= cnt) return;
+    for (int k = 256 * (wave >> 2) + 4 * lane; k < keys; k += 64 * waves) {
+        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        with_taps(S2, [&](auto count) {
+            for (int j = 0; j < R2; ++j) taps4<decltype(count)::value>(c, rows + (u * R2 + j) * stride + k - left, w2 + (u * R2 + j) * sp, S2);
+        });
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = s.base + k + e >= s.lo ? c[e] : 0.0f;
+        *reinterpret_cast<f32x4 *>(m.p1 + ((int64_t)b * H + o0 + u) * m.span + k) = f32x4{c[0], c[1], c[2], c[3]};
+    }
+}
+
 // ---- mixing behind the softmax and P V: V once ----
 // POST: p1 has been through the second conv; else the heads' probabilities are formed here, from scores and statistics.
 template <typename T, int D, int NT, int GW, bool POST>
@@ -406,7 +518,7 @@ template <typename T, int D> __global__ __launch_bounds__(256) void decode_sum_k
 struct plan {
     cut t, v;                                         // items of the scores and of the values kernel
     int gw, lds;                                      // scores
-    int span, chunk, chunks, v_gw, v_lds, mix_lds, post_waves, post_lds;
+    int span, chunk, chunks, v_gw, v_lds, mix_lds, post_waves, post_lds, short_kq, short_lds;   // short_kq: 256s of keys in a short row, or 0
     int64_t s1, s2, stats, p1, part, total;           // workspace, in floats
 };
 
@@ -431,6 +543,9 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
     p.mix_lds = DECODE_WAVES * pre_group * 16;
     for (p.post_waves = 4; p.post_waves > 1 && p.post_waves * post_floats(R2, S2) * 4 > 64 << 10;) p.post_waves >>= 1;
     p.post_lds = p.post_waves * post_floats(R2, S2) * 4;
+    p.short_kq = !post_conv ? 0 : p.span == 256 ? 1 : p.span == 512 ? 2 : 0;
+    p.short_lds = short_floats(R2, S2, pre_group, p.short_kq) * 4;
+    if (p.short_lds > 160 << 10) p.short_kq = 0;
     p.v_gw = share % 4 == 0 ? 4 : share % 2 == 0 ? 2 : 1;
     p.v = cut_of(span_of(longest, window, 1), B, H / p.v_gw, most_tiles(D * size), 1024, true);
     p.v_lds = (2 * up16(p.v_gw * post_group) + DECODE_WAVES * p.v_gw * (16 * p.v.nt + D)) * 4;
@@ -486,11 +601,19 @@ template <typename T, int D> int launch_all(const mta_args &m, const plan &p, hi
     if constexpr (MOST >= 4)
         if (p.t.nt == 4) e = launch_scores_rows<T, D, 4>(m, p, st);
     if (e) return e;
-    if ((e = allow_lds(decode_mix_kernel, p.mix_lds))) return e;
-    hipLaunchKernelGGL(decode_mix_kernel, dim3((unsigned)m.R2, (unsigned)p.chunks, slots), dim3(256), p.mix_lds, st, m);
-    if (m.w2) {
-        if ((e = allow_lds(decode_post_kernel, p.post_lds))) return e;
-        hipLaunchKernelGGL(decode_post_kernel, dim3((heads + p.post_waves - 1) / p.post_waves, (unsigned)((p.span + post_keys(m.S2) - 1) / post_keys(m.S2)), slots), dim3(64 * p.post_waves), p.post_lds, st, m);
+    if (p.short_kq) {
+        const dim3 grid(heads / m.pre_group * ((m.pre_group + 3) / 4), slots);
+        auto kern = p.short_kq == 1 ? decode_mix_post_kernel<1> : decode_mix_post_kernel<2>;
+        if ((e = allow_lds(kern, p.short_lds))) return e;
+        hipLaunchKernelGGL(kern, grid, dim3(m.R2 <= 8 ? 512 : 1024), p.short_lds, st, m);
+    } else {
+        if ((e = allow_lds(decode_mix_kernel, p.mix_lds))) return e;
+        hipLaunchKernelGGL(decode_mix_kernel, dim3((unsigned)m.R2, (unsigned)p.chunks, slots), dim3(256), p.mix_lds, st, m);
+        if (m.w2) {
+            if ((e = allow_lds(decode_post_kernel, p.post_lds))) return e;
+            const dim3 grid((heads + p.post_waves - 1) / p.post_waves, (unsigned)((p.span + post_keys(m.S2) - 1) / post_keys(m.S2)), slots);
+            hipLaunchKernelGGL(decode_post_kernel, grid, dim3(64 * p.post_waves), p.post_lds, st, m);
+        }
     }
     e = MTA_ERR_UNSUPPORTED;
     if (p.v.nt == 1) e = launch_values_conv<T, D, 1>(m, p, st);

@@ -241,6 +241,46 @@ def test_mta_long():
         check(got[b, 0], *seq.want(b, w, d ** -0.5, pre=pre, w2=w2, post=post), what=f"slot {b}")
 
 
+@pytest.mark.parametrize("h,r2,s2,group", [(8, 3, 3, 0), (6, 2, 5, 3), (5, 7, 7, 5), (9, 9, 4, 1), (12, 12, 11, 6), (4, 1, 16, 0), (4, 32, 2, 2), (2, 17, 63, 0), (7, 6, 1, 0)])
+@pytest.mark.parametrize("length", [2, 256, 257, 300, 505, 512, 513, 700])
+def test_mta_rows_of_few_keys(h, r2, s2, group, length):
+    """Rows around the lengths at which the stages behind the scores are laid out in another way; heads that no four divide."""
+    d, dtype = 64, torch.float32
+    print(f"mta decode h={h} {r2}x{s2} group={group} {length}", flush=True)
+    seq = Sequences([length - 1, length // 2, 0], h, h, d, dtype, 32, r2 + 1, scatter=False)
+    w, w2 = conv_weight(h, 2, 3, dtype, seq.gen), conv_weight(h, r2, s2, dtype, seq.gen)
+    pre, post = head_weight(h, group or h, dtype, seq.gen), head_weight(h, group or h, dtype, seq.gen)
+    plain = mta_module(w, None, w2, None, pre_head_identity=True, post_head_identity=True)
+    full = mta_module(w, pre, w2, post, **(dict(pre_head_group=group, post_head_group=group) if group else {}))
+    seq.feed([1, 1, 0])
+    got, got2 = plain.decode(seq.cache), full.decode(seq.cache)
+    for b in range(2):
+        check(got[b, 0], *seq.want(b, w, d ** -0.5, w2=w2), what=f"slot {b}")
+        check(got2[b, 0], *seq.want(b, w, d ** -0.5, pre=pre, w2=w2, post=post), what=f"slot {b}")
+    assert not got[2].any() and not got2[2].any()
+    for window in (3, 400):
+        got2 = full.decode(seq.cache, window=window)
+        for b in range(2):
+            check(got2[b, 0], *seq.want(b, w, d ** -0.5, pre=pre, w2=w2, post=post, window=window), what=f"slot {b}, window {window}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nothing_added_yet(dtype):
+    """A new cache, one whose slots all sit the step out, one that was emptied: zeros."""
+    seq = Sequences([0, 0], 4, 2, 64, dtype, 16, 8)
+    w, w2 = conv_weight(4, 3, 3, dtype, seq.gen), conv_weight(4, 3, 3, dtype, seq.gen)
+    pre = head_weight(4, 4, dtype, seq.gen)
+    conv, full = conv_module(w), mta_module(w, pre, w2, pre)
+    for counts in (None, [0, 0], [3, 5], [0, 0]):
+        if counts:
+            seq.cache.extend(counts) if not any(counts) else seq.feed(counts)
+        got, got2 = conv.decode(seq.cache), full.decode(seq.cache)
+        assert got.isfinite().all() and got2.isfinite().all() and got.any().item() == got2.any().item() == any(counts or [])
+    for b in range(2):
+        seq.cache.free(b)
+    assert not conv.decode(seq.cache).any() and not full.decode(seq.cache).any()
+
+
 def test_mta_weights_of_other_dtypes():
     h, d = 4, 64
     seq = Sequences([77], h, h, d, torch.float16, 16, 5)
