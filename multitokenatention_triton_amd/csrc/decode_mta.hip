@@ -217,60 +217,78 @@ template <int PARTS> __device__ __forceinline__ float2 row_statistics(const floa
 // its own part of LDS.
 __host__ __device__ __forceinline__ int post_left(int S2) { return ((S2 - 1) / 2 + 3) & ~3; }
 __host__ __device__ __forceinline__ int post_keys(int S2) { return 256 - post_left(S2) - ((S2 - 1 - (S2 - 1) / 2 + 3) & ~3); }   // results
+__host__ __device__ __forceinline__ int post_blocks(int span, int S2) { return (span + post_keys(S2) - 1) / post_keys(S2); }
 constexpr int POST_STRIDE = 256 + 12;
 __host__ __device__ __forceinline__ int post_floats(int R2, int S2) { return 2 * up16(R2) + R2 * (((S2 + 3) & ~3) + POST_STRIDE); }
 
-__global__ __launch_bounds__(256) void decode_post_kernel(const mta_args m)
+// SPLIT: the four wavefronts of a workgroup take the same keys of one head and deal its rows out among them, which shortens the chain of a wavefront
+// and costs four times the starts and a sum: for more than eight rows, and for fewer while the workgroups are no more than 192 to a row.  All kernels
+// of a call, us, split | not (slots x heads, keys, R2 x S2): 1 x 8, 1500: 3 x 3 21.6 | 22.6, 11 x 15 22.4 | 27.7; 16 x 16, 600 (768 workgroups):
+// 3 x 3 33.9 | 33.8, 6 x 9 30.8 | 31.6, 11 x 15 33.2 | 37.2; 16 x 16, 4000 (4352): 3 x 3 86.7 | 82.2, 6 x 9 95.8 | 94.0, 11 x 15 111.7 | 117.4.
+template <bool SPLIT> __global__ __launch_bounds__(256) void decode_post_kernel(const mta_args m)
 {
     extern __shared__ __align__(16) float lds[];
     const int b = blockIdx.z, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), H = m.d.heads;
-    const int h = blockIdx.x * (blockDim.x >> 6) + wave;
+    const int h = SPLIT ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + wave;
     const slot_step s = step_of(m, b);
     const int k0 = s.base + blockIdx.y * post_keys(m.S2);
-    if (h >= H || s.n <= 0 || k0 >= s.n) return;   // (nothing below waits for another wavefront)
-    const int left = (m.S2 - 1) / 2, left4 = post_left(m.S2), shift = left & 3, taps = m.R2 * m.S2, sp = (m.S2 + 3) & ~3;
-    float *const mine = lds + wave * post_floats(m.R2, m.S2), *const w = mine + 2 * up16(m.R2), *const p = w + m.R2 * sp;
+    if (h >= H || s.n <= 0 || k0 >= s.n) return;   // (SPLIT: all four wavefronts or none; else nothing below waits for another one)
+    const int r0 = SPLIT ? wave * m.R2 / 4 : 0, R2 = (SPLIT ? (wave + 1) * m.R2 / 4 : m.R2) - r0;   // rows
+    const int left = (m.S2 - 1) / 2, left4 = post_left(m.S2), shift = left & 3, taps = R2 * m.S2, sp = (m.S2 + 3) & ~3;
+    float *const mine = lds + wave * post_floats(SPLIT ? (m.R2 + 3) / 4 : R2, m.S2), *const w = mine + 2 * up16(R2), *const p = w + R2 * sp;
     float2 *const stat = reinterpret_cast<float2 *>(mine);
-    const int64_t row0 = ((int64_t)b * H + h) * m.R2;
+    const int64_t row0 = ((int64_t)b * H + h) * m.R2 + r0;
     const int chunks = (s.n - s.base + m.chunk - 1) / m.chunk;
     // (loads first: scores, which do not wait for the statistics, then weights and statistics)
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = SPLIT ? 4 : 8;
     const int key0 = k0 - left4 + 4 * lane;
     const float *const sc = (m.w_pre ? m.s2 : m.s1) + row0 * m.span + (key0 >= s.base && key0 < s.n ? key0 - s.base : 0);
     f32x4 x[AHEAD];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) x[j] = *reinterpret_cast<const f32x4 *>(sc + (int64_t)(j < m.R2 ? j : 0) * m.span);
+    for (int j = 0; j < AHEAD; ++j) x[j] = *reinterpret_cast<const f32x4 *>(sc + (int64_t)(j < R2 ? j : 0) * m.span);
 #pragma unroll 4
-    for (int t = lane; t < taps; t += 64) w[t / m.S2 * sp + t % m.S2] = load_any(m.w2, m.d.w_dtype, (int64_t)h * taps + t);
-    for (int t = lane; t < m.R2 * 8; t += 64) {
+    for (int t = lane; t < taps; t += 64) w[t / m.S2 * sp + t % m.S2] = load_any(m.w2, m.d.w_dtype, ((int64_t)h * m.R2 + r0) * m.S2 + t);
+    for (int t = lane; t < R2 * 8; t += 64) {
         const float2 st = row_statistics<8>(m.stats + (row0 + t / 8) * m.chunks * 2, chunks, t % 8);
         if (t % 8 == 0) stat[t / 8] = st;
     }
     wave_sync();
-    for (int j0 = 0; j0 < m.R2; j0 += AHEAD) {
+    for (int j0 = 0; j0 < R2; j0 += AHEAD) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            if (j0 + j >= m.R2) break;
-            const int pos = row_pos(m, s.n, j0 + j);
+            if (j0 + j >= R2) break;
+            const int pos = row_pos(m, s.n, r0 + j0 + j);
             const float2 st = stat[j0 + j];
             float *const to = p + (j0 + j) * POST_STRIDE + shift + 4 * lane;   // (the taps of a lane's keys begin on 16 bytes)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 to[e] = key0 + e >= s.base && sees(m, pos, key0 + e) ? __builtin_amdgcn_exp2f(fmaf(x[j][e], LOG2E, -st.x)) * st.y : 0.0f;
         }
-        if (j0 + AHEAD < m.R2) {
+        if (j0 + AHEAD < R2) {
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) x[j] = *reinterpret_cast<const f32x4 *>(sc + (int64_t)(j0 + AHEAD + j < m.R2 ? j0 + AHEAD + j : 0) * m.span);
+            for (int j = 0; j < AHEAD; ++j) x[j] = *reinterpret_cast<const f32x4 *>(sc + (int64_t)(j0 + AHEAD + j < R2 ? j0 + AHEAD + j : 0) * m.span);
         }
     }
     wave_sync();
     const int key = k0 + 4 * lane;
-    if (4 * lane >= post_keys(m.S2) || key >= s.n) return;
+    const bool there = 4 * lane < post_keys(m.S2) && key < s.n;
+    if (!SPLIT && !there) return;
     float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const float *const from = p + shift + 4 * lane + left4 - left;
-    with_taps(m.S2, [&](auto count) {
-        for (int j = 0; j < m.R2; ++j) taps4<decltype(count)::value>(c, from + j * POST_STRIDE, w + j * sp, m.S2);
-    });
+    if (there)
+        with_taps(m.S2, [&](auto count) {
+            for (int j = 0; j < R2; ++j) taps4<decltype(count)::value>(c, from + j * POST_STRIDE, w + j * sp, m.S2);
+        });
+    if constexpr (SPLIT) {
+        __syncthreads();
+        *reinterpret_cast<f32x4 *>(lds + 256 * wave + 4 * lane) = f32x4{c[0], c[1], c[2], c[3]};
+        __syncthreads();
+        if (wave || !there) return;
+#pragma unroll
+        for (int o = 1; o < 4; ++o)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] += lds[256 * o + 4 * lane + e];
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) c[e] = key + e >= s.lo ? c[e] : 0.0f;
     *reinterpret_cast<f32x4 *>(m.p1 + ((int64_t)b * H + h) * m.span + (key - s.base)) = f32x4{c[0], c[1], c[2], c[3]};
@@ -518,7 +536,7 @@ template <typename T, int D> __global__ __launch_bounds__(256) void decode_sum_k
 struct plan {
     cut t, v;                                         // items of the scores and of the values kernel
     int gw, lds;                                      // scores
-    int span, chunk, chunks, v_gw, v_lds, mix_lds, post_waves, post_lds, short_kq, short_lds;   // short_kq: 256s of keys in a short row, or 0
+    int span, chunk, chunks, v_gw, v_lds, mix_lds, post_waves, post_lds, post_split, short_kq, short_lds;   // short_kq: 256s of keys in a short row, or 0
     int64_t s1, s2, stats, p1, part, total;           // workspace, in floats
 };
 
@@ -543,6 +561,8 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
     p.mix_lds = DECODE_WAVES * pre_group * 16;
     for (p.post_waves = 4; p.post_waves > 1 && p.post_waves * post_floats(R2, S2) * 4 > 64 << 10;) p.post_waves >>= 1;
     p.post_lds = p.post_waves * post_floats(R2, S2) * 4;
+    p.post_split = R2 > 1 && (R2 > 8 || H * B * post_blocks(p.span, S2) <= 192 * R2);
+    if (p.post_split) p.post_waves = 4, p.post_lds = 16 * post_floats((R2 + 3) / 4, S2);
     p.short_kq = !post_conv ? 0 : p.span == 256 ? 1 : p.span == 512 ? 2 : 0;
     p.short_lds = short_floats(R2, S2, pre_group, p.short_kq) * 4;
     if (p.short_lds > 160 << 10) p.short_kq = 0;
@@ -610,9 +630,11 @@ template <typename T, int D> int launch_all(const mta_args &m, const plan &p, hi
         if ((e = allow_lds(decode_mix_kernel, p.mix_lds))) return e;
         hipLaunchKernelGGL(decode_mix_kernel, dim3((unsigned)m.R2, (unsigned)p.chunks, slots), dim3(256), p.mix_lds, st, m);
         if (m.w2) {
-            if ((e = allow_lds(decode_post_kernel, p.post_lds))) return e;
-            const dim3 grid((heads + p.post_waves - 1) / p.post_waves, (unsigned)((p.span + post_keys(m.S2) - 1) / post_keys(m.S2)), slots);
-            hipLaunchKernelGGL(decode_post_kernel, grid, dim3(64 * p.post_waves), p.post_lds, st, m);
+            auto kern = p.post_split ? decode_post_kernel<true> : decode_post_kernel<false>;
+            if ((e = allow_lds(kern, p.post_lds))) return e;
+            const int at_once = p.post_split ? 1 : p.post_waves;
+            const dim3 grid((heads + at_once - 1) / at_once, (unsigned)post_blocks(p.span, m.S2), slots);
+            hipLaunchKernelGGL(kern, grid, dim3(64 * p.post_waves), p.post_lds, st, m);
         }
     }
     e = MTA_ERR_UNSUPPORTED;
