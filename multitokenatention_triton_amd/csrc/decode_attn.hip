@@ -139,26 +139,37 @@ __global__ __launch_bounds__(256, 2) void conv_attn_decode_kernel(const decode_a
     }
 }
 
-// The items of one (slot, head), brought to one reference and added up, always in the same order.
+// The items of one (slot, head), brought to one reference and added up, always in the same order.  A lane takes four elements of every PARTS-th
+// item; the first AHEAD of its items are on their way while the factors are formed (a call over 8 slots of up to 4k keys, 32 heads 26.0 -> 24.7 us).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a, int shift)
 {
-    constexpr int PARTS = 256 / D;
-    __shared__ float so[PARTS][D], factor[64];
-    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D, lane = threadIdx.x & 63;
+    constexpr int PARTS = 1024 / D, AHEAD = 4;
+    __shared__ __align__(16) float so[PARTS][D];
+    __shared__ float factor[64];
+    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % (D / 4) * 4, part = threadIdx.x / (D / 4), lane = threadIdx.x & 63;
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
     const shares sh(a, 0, shift, false, lane);
     const work_item it = item_of(sh, 0, b, lane);
     const int items = it.count;
     if (items == 1) return;   // (that item wrote the result)
-    const int64_t at = (int64_t)it.first * a.heads + h;
-    const float *o = a.ws + at * D;
+    const int64_t at = (int64_t)it.first * a.heads + h, stride = (int64_t)a.heads * D;
+    const float *o = a.ws + at * D + d;
     const float2 *ml = reinterpret_cast<const float2 *>(a.ws + stats_offset(a.items, a.heads, D)) + at;
+    f32x4 first[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) first[u] = *reinterpret_cast<const f32x4 *>(o + (part + u * PARTS < items ? part + u * PARTS : 0) * stride);
     float top = -INFINITY;
     for (int i = lane; i < items; i += 64) top = fmaxf(top, ml[(int64_t)i * a.heads].x);
     top = wave_max(top);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, total = 0.0f;
+    float total = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    const auto add = [&](int i, const f32x4 &x) {
+        const float f = factor[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, x[e], sum[e]);
+    };
     for (int i0 = 0; i0 < items; i0 += 64) {   // (factors of 64 items at a time; all wavefronts form the same ones)
         const float2 x = i0 + lane < items ? ml[(int64_t)(i0 + lane) * a.heads] : make_float2(-INFINITY, 0.0f);
         const float f = __builtin_amdgcn_exp2f(x.x - ref);
@@ -167,16 +178,23 @@ __global__ __launch_bounds__(256) void conv_attn_join_kernel(const decode_args a
         if (threadIdx.x < 64) factor[lane] = f;
         __syncthreads();
         const int most = items - i0 < 64 ? items - i0 : 64;
-#pragma unroll 8
-        for (int i = part; i < most; i += PARTS) sum = fmaf(factor[i], o[(int64_t)(i0 + i) * a.heads * D + d], sum);
+        int i = part;
+        if (i0 == 0) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u, i += PARTS)
+                if (i < most) add(i, first[u]);
+        }
+#pragma unroll 4
+        for (; i < most; i += PARTS) add(i, *reinterpret_cast<const f32x4 *>(o + (i0 + i) * stride));
     }
     total = wave_sum(total);
-    so[part][d] = sum;
+    *reinterpret_cast<f32x4 *>(&so[part][d]) = sum;
     __syncthreads();
-    if (part != 0) return;
+    if (threadIdx.x >= D) return;
+    float all = 0.0f;
 #pragma unroll
-    for (int i = 1; i < PARTS; ++i) sum += so[i][d];
-    out[d] = from_float<T>(sum / total);
+    for (int i = 0; i < PARTS; ++i) all += so[i][threadIdx.x];
+    out[threadIdx.x] = from_float<T>(all / total);
 }
 
 struct plan { cut t; int gw, lds; };

@@ -511,25 +511,26 @@ __global__ __launch_bounds__(256) void decode_values_kernel(const mta_args m)
 
 template <typename T, int D> __global__ __launch_bounds__(256) void decode_sum_kernel(const mta_args m)
 {
-    constexpr int PARTS = 256 / D;
-    __shared__ float so[PARTS][D];
+    constexpr int PARTS = 1024 / D;   // (four elements to a lane)
+    __shared__ __align__(16) float so[PARTS][D];
     decode_args a = m.d;
     a.target = m.v_target, a.least = m.v_least, a.items = m.v_items;
-    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, part = threadIdx.x / D, lane = threadIdx.x & 63;
+    const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x % (D / 4) * 4, part = threadIdx.x / (D / 4), lane = threadIdx.x & 63;
     const shares sh(a, m.R2 - 1, m.v_shift, true, lane);
     const work_item it = item_of(sh, 0, b, lane);
     if (it.count == 1) return;   // (that item wrote the result)
     T *const out = (T *)a.o + ((int64_t)b * a.heads + h) * D;
     const float *o = m.part + ((int64_t)it.first * a.heads + h) * D + d;
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int i = part; i < it.count; i += PARTS) sum += o[(int64_t)i * a.heads * D];
-    so[part][d] = sum;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i = part; i < it.count; i += PARTS) sum += *reinterpret_cast<const f32x4 *>(o + (int64_t)i * a.heads * D);
+    *reinterpret_cast<f32x4 *>(&so[part][d]) = sum;
     __syncthreads();
-    if (part != 0) return;
+    if (threadIdx.x >= D) return;
+    float all = 0.0f;
 #pragma unroll
-    for (int i = 1; i < PARTS; ++i) sum += so[i][d];
-    out[d] = from_float<T>(sum);
+    for (int i = 0; i < PARTS; ++i) all += so[i][threadIdx.x];
+    out[threadIdx.x] = from_float<T>(all);
 }
 
 // ---- host side ----
