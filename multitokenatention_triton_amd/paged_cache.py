@@ -18,7 +18,7 @@ A step::
 read of it - the table and two numbers per slot - is copied to the device on the current stream.
 The kernels never wait for the host, and a step may be captured into a graph (``append`` and
 ``decode``; not ``extend``, which is called between replays: the graph reads the table anew every time
-and has to be captured with as many new tokens as a slot gets at most).  All calls on one cache
+and has to be captured with as many new tokens as a slot gets at most; ``mark_appended`` tells the host of a replay).  All calls on one cache
 belong on one stream, or are ordered by the caller.
 """
 from __future__ import annotations
@@ -73,6 +73,7 @@ class PagedCache:
         self._host = self._plan.cpu()
         self._host_state, self._host_table = self._host[:2 * n].view(2, n), self._host[2 * n:].view(n, max_pages)
         self._lengths, self._added = [0] * n, [0] * n
+        self._due = False          # the tokens of the last extend are in no page yet, as far as the host knows
         self._pages: List[List[int]] = [[] for _ in range(n)]
         self._uses = [0] * k.size(0)
         self._free = list(range(k.size(0)))    # a heap: the lowest page first
@@ -177,8 +178,8 @@ class PagedCache:
         self._pages[slot], self._lengths[slot], self._added[slot] = [], 0, 0
 
     def extend(self, counts: Union[int, Sequence[int]]) -> None:
-        """``counts`` more positions for every slot (a number, or one per slot; 0: the slot sits the next steps out).  Raises, and
-        changes nothing, where pages or the table run out."""
+        """``counts`` more positions for every slot (a number, or one per slot; 0: the slot sits the next steps out).  ``append`` fills
+        those of the last call only, so it comes before the next one.  Raises, and changes nothing, where pages or the table run out."""
         self._eager("extend")
         counts = [counts] * self.n_slots if isinstance(counts, int) else [int(c) for c in counts]
         if len(counts) != self.n_slots or any(c < 0 for c in counts):
@@ -198,6 +199,7 @@ class PagedCache:
                 self._pages[slot].append(p)
             self._lengths[slot] += c
             self._added[slot] = c
+        self._due = True
         self._upload([slot for slot, w in enumerate(want) if w])
 
     def free(self, slot: int) -> None:
@@ -214,19 +216,30 @@ class PagedCache:
         if xk.dim() == 4 and xk.size(2) < max(self._added):
             raise ValueError(f"extend made room for up to {max(self._added)} tokens, append got {xk.size(2)}")
         _lib.host().cache_append(self.k, self.v, self.q, self.table, self.state, xq, xk, xv)
+        if not torch.cuda.is_current_stream_capturing():
+            self._due = False
+
+    def mark_appended(self) -> None:
+        """Says that the tokens of the last ``extend`` are in their pages: after the replay of a graph that appends them, which the
+        host does not see, or where something else wrote them.  ``append`` says so by itself."""
+        self._due = False
 
     def fork(self, source: int, targets: Union[int, Sequence[int]]) -> None:
         """Makes ``targets`` copies of slot ``source`` (a beam that splits, samples of one prompt): whole pages are shared, the page
         that is being filled and the ring of queries are copied.  What the targets held is released.  They sit steps out
-        until they are extended."""
+        until they are extended.  The source's tokens have to be in their pages: between ``extend`` and ``append`` a fork is
+        refused (``mark_appended``, where a replayed graph appended them)."""
         self._eager("fork")
         targets = [targets] if isinstance(targets, int) else list(targets)
         for slot in [source] + targets:
             self._slot(slot)
         if source in targets or len(set(targets)) < len(targets):
             raise ValueError(f"fork takes different targets, and none that is the source: {source} to {targets}")
+        if targets and self._due and self._added[source]:
+            # (their copies would be taken now, and the append to come writes the source's pages alone)
+            raise RuntimeError(f"slot {source} holds {self._added[source]} tokens that have not been appended yet: append them before a fork"
+                               + ("" if self.k.is_cuda else f" (the cache lives on {self.k.device}: append has no CPU path)"))
         n, page = self._lengths[source], self.page_size
-        # (a page whose tokens are still to be appended counts as being filled)
         whole = (n - self._added[source]) // page if n else 0
         shared, partial = self._pages[source][:whole], self._pages[source][whole:]
         going = {}

@@ -88,6 +88,39 @@ def test_fork_shares_whole_pages():
             c.fork(0, targets)
 
 
+def test_fork_waits_for_append():
+    """Between extend and append a slot counts tokens that are in no page yet: a copy of it would never get them."""
+    for counts in ([20, 0, 0], [32, 0, 0]):
+        c = cache()
+        c.extend([0, 40, 0])
+        c.extend(counts)
+        for targets in (1, [2], [1, 2]):
+            with pytest.raises(RuntimeError, match=f"{counts[0]} tokens.*not been appended"):
+                c.fork(0, targets)
+            consistent(c)
+            assert c.lengths == [counts[0], 40, 0] and c._added == counts
+        c.fork(1, [])
+        c.fork(2, [1])                  # (a slot that got none can be copied all the while)
+        consistent(c)
+        assert c.lengths == [counts[0], 0, 0]
+
+
+def test_mark_appended():
+    """What a replayed graph appended, the cache is told of."""
+    c = cache()
+    c.extend([32, 0, 0])
+    c.mark_appended()
+    c.extend([0, 0, 0])
+    c.fork(0, 1)
+    consistent(c)
+    c.extend([16, 0, 0])                # ... and that holds for one extend
+    with pytest.raises(RuntimeError, match="not been appended"):
+        c.fork(0, 2)
+    c.free(0)
+    c.fork(0, 2)
+    assert c.lengths == [0, 32, 0]
+
+
 def test_compact_without_moves():
     c = cache()
     assert c.compact() == 0

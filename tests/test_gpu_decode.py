@@ -327,6 +327,55 @@ def test_prompt_then_tokens_then_fork_then_compact():
     step([5, 1, 1, 0])
 
 
+def test_fork_between_extend_and_append():
+    """Refused while the source's tokens are in no page; once appended - by a call or by a graph that the cache is told of - the copy has them."""
+    h, d, dtype = 4, 64, torch.float32
+    seq = Sequences([35, 3, 0], h, h, d, dtype, 16, 4, scatter=False)
+    w = conv_weight(h, 4, 5, dtype, seq.gen)
+    module = conv_module(w)
+    n = 35
+
+    def same(slot):
+        for x in (seq.q, seq.k, seq.v):
+            x[slot, :, :n] = x[0, :, :n]
+
+    def new():
+        return [x[:, :, n - 1:n].cuda() for x in (seq.q, seq.k, seq.v)]
+
+    def step():
+        seq.feed([1, 1, 1])
+        got = module.decode(seq.cache)
+        for b in range(3):
+            check(got[b, :, 0], *seq.want(b, w, d ** -0.5), what=f"slot {b}")
+
+    seq.cache.extend([1, 0, 0])
+    n += 1
+    with pytest.raises(RuntimeError, match="not been appended"):
+        seq.cache.fork(0, 2)
+    assert seq.cache.lengths == [36, 3, 0]
+    seq.cache.append(*new())
+    seq.cache.fork(0, 2)
+    same(2)
+    step()
+    n += 1
+    static = [x.clone() for x in new()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        seq.cache.append(*static)
+    seq.cache.extend([1, 0, 0])
+    n += 1
+    for x, y in zip(static, new()):
+        x.copy_(y)
+    graph.replay()
+    with pytest.raises(RuntimeError, match="not been appended"):
+        seq.cache.fork(0, 1)
+    seq.cache.mark_appended()
+    seq.cache.fork(0, 1)
+    same(1)
+    step()
+
+
 def test_adopted_cache():
     h, d, dtype = 4, 64, torch.bfloat16
     seq = Sequences([50, 20], h, h, d, dtype, 16, 3, scatter=True)
