@@ -74,6 +74,7 @@ class PagedCache:
         self._host_state, self._host_table = self._host[:2 * n].view(2, n), self._host[2 * n:].view(n, max_pages)
         self._lengths, self._added = [0] * n, [0] * n
         self._due = False          # the tokens of the last extend are in no page yet, as far as the host knows
+        self._shared = False       # ... are in pages that a fork has shared since
         self._pages: List[List[int]] = [[] for _ in range(n)]
         self._uses = [0] * k.size(0)
         self._free = list(range(k.size(0)))    # a heap: the lowest page first
@@ -140,7 +141,7 @@ class PagedCache:
     @property
     def longest(self) -> int:
         """What sizes a decode: the longest slot; while a graph is captured, what the table has room for."""
-        if self.k.is_cuda and torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             return self.table.size(1) * self.page_size
         return max(1, max(self._lengths))
 
@@ -149,8 +150,11 @@ class PagedCache:
             raise ValueError(f"a slot is a number from 0 to {self.n_slots - 1}, got {slot!r}")
         return slot
 
+    def _capturing(self) -> bool:
+        return self.k.is_cuda and torch.cuda.is_current_stream_capturing()
+
     def _eager(self, what: str) -> None:
-        if self.k.is_cuda and torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             raise RuntimeError(f"{what} is host bookkeeping and cannot be captured into a graph: call it between replays")
 
     def _upload(self, slots=(), everything: bool = False) -> None:
@@ -199,7 +203,7 @@ class PagedCache:
                 self._pages[slot].append(p)
             self._lengths[slot] += c
             self._added[slot] = c
-        self._due = True
+        self._due, self._shared = True, False
         self._upload([slot for slot, w in enumerate(want) if w])
 
     def free(self, slot: int) -> None:
@@ -213,10 +217,12 @@ class PagedCache:
         """The tokens of the last ``extend``: (slots, n_heads, n, D) queries, (slots, kv_heads, n, D) keys and values, any strides
         with contiguous rows; slot b takes its first ``added[b]`` tokens, n is at least the most of them.  One kernel
         (``mta_cache_append``)."""
+        if self._shared and not self._capturing():
+            raise RuntimeError("the tokens of the last extend lie in pages that are shared since a fork: extend before the next append")
         if xk.dim() == 4 and xk.size(2) < max(self._added):
             raise ValueError(f"extend made room for up to {max(self._added)} tokens, append got {xk.size(2)}")
         _lib.host().cache_append(self.k, self.v, self.q, self.table, self.state, xq, xk, xv)
-        if not torch.cuda.is_current_stream_capturing():
+        if not self._capturing():
             self._due = False
 
     def mark_appended(self) -> None:
@@ -228,7 +234,8 @@ class PagedCache:
         """Makes ``targets`` copies of slot ``source`` (a beam that splits, samples of one prompt): whole pages are shared, the page
         that is being filled and the ring of queries are copied.  What the targets held is released.  They sit steps out
         until they are extended.  The source's tokens have to be in their pages: between ``extend`` and ``append`` a fork is
-        refused (``mark_appended``, where a replayed graph appended them)."""
+        refused (``mark_appended``, where a replayed graph appended them), and what is appended behind it, by a call or by a
+        replay, is the tokens of a later ``extend``."""
         self._eager("fork")
         targets = [targets] if isinstance(targets, int) else list(targets)
         for slot in [source] + targets:
@@ -240,7 +247,7 @@ class PagedCache:
             raise RuntimeError(f"slot {source} holds {self._added[source]} tokens that have not been appended yet: append them before a fork"
                                + ("" if self.k.is_cuda else f" (the cache lives on {self.k.device}: append has no CPU path)"))
         n, page = self._lengths[source], self.page_size
-        whole = (n - self._added[source]) // page if n else 0
+        whole = n // page
         shared, partial = self._pages[source][:whole], self._pages[source][whole:]
         going = {}
         for slot in targets:
@@ -258,6 +265,8 @@ class PagedCache:
                 self._uses[p] += 1
             pairs += list(zip(partial, copies))
             self._pages[slot], self._lengths[slot], self._added[slot] = shared + copies, n, 0
+        if targets and whole * page > n - self._added[source]:
+            self._shared = True
         self._upload(targets)
         if pairs:
             ops.cache_copy_pages(self.k, self.v, pairs)

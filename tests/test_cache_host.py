@@ -105,6 +105,25 @@ def test_fork_waits_for_append():
         assert c.lengths == [counts[0], 0, 0]
 
 
+def test_fork_of_a_new_prompt():
+    """What has been appended is shared, however new it is."""
+    c = cache(n_pages=4)
+    c.extend([48, 0, 0])
+    c.mark_appended()
+    c.fork(0, [1, 2])                   # (copies would need six pages, one is free)
+    consistent(c)
+    assert c.pages_of(0) == c.pages_of(1) == c.pages_of(2) == [0, 1, 2] and c.free_pages == 1 and c.lengths == [48, 48, 48]
+    assert c._added == [48, 0, 0]       # (the source's newest row can still be computed)
+    x = torch.zeros(3, 4, 48, 64)
+    with pytest.raises(RuntimeError, match="shared"):
+        c.append(x, x[:, :2], x[:, :2])  # those tokens are the targets' as well now
+    c.extend([0, 0, 1])
+    consistent(c)
+    assert c.pages_of(2) == [0, 1, 2, 3]
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        c.append(x, x[:, :2], x[:, :2])
+
+
 def test_mark_appended():
     """What a replayed graph appended, the cache is told of."""
     c = cache()

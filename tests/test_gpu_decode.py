@@ -376,6 +376,29 @@ def test_fork_between_extend_and_append():
     step()
 
 
+@pytest.mark.parametrize("n", [96, 100, 15])
+def test_fork_of_a_new_prompt(n):
+    """Samples of one prompt, straight after its append: whole pages are shared, one page is copied at most; all go on alone."""
+    h, d, dtype, page = 4, 64, torch.bfloat16, 16
+    seq = Sequences([n, 0, 0, 0], h, 2, d, dtype, page, 5, n_pages=n // page + 8, scatter=False)
+    w = conv_weight(h, 5, 7, dtype, seq.gen)
+    module = conv_module(w)
+    free = seq.cache.free_pages
+    seq.cache.fork(0, [1, 2, 3])
+    assert all(seq.cache.pages_of(b)[:n // page] == seq.cache.pages_of(0)[:n // page] for b in range(4))
+    assert seq.cache.free_pages == free - 3 * (n % page > 0)
+    for x in (seq.q, seq.k, seq.v):
+        x[1:, :, :n] = x[:1, :, :n]
+    got = module.decode(seq.cache)
+    check(got[0, :, 0], *seq.want(0, w, d ** -0.5))
+    assert not got[1:].any()
+    for _ in range(2):
+        seq.feed([1, 1, 1, 1])
+        got = module.decode(seq.cache)
+        for b in range(4):
+            check(got[b, :, 0], *seq.want(b, w, d ** -0.5), what=f"slot {b}")
+
+
 def test_adopted_cache():
     h, d, dtype = 4, 64, torch.bfloat16
     seq = Sequences([50, 20], h, h, d, dtype, 16, 3, scatter=True)
