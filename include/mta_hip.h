@@ -536,7 +536,7 @@ int mta_cache_copy_pages(void *k, void *v, int64_t n_pages, int64_t page_bytes, 
  *   o[b,h] = softmax_k( scale * sum_{r,t} w[h,r,t] raw_{p-R+1+r}[k+t-(S-1)/2] ) V,   raw_i[k] = q_i . k_k, or 0 where row i does not see
  * key k: it sees max(0, i - window + 1) .. i (window = 0: from key 0 on).  o is (slots, heads, head_dim), zeros for slots that sit out.
  * query_rows >= R.  Everything between the inputs and o is held in fp32.  longest: no slot holds more tokens (state counted in full);
- * it sizes the grid and the workspace (8-byte aligned).  The workspace call returns bytes, or an error code. */
+ * it sizes the grid and the workspace (16-byte aligned).  The workspace call returns bytes, or an error code. */
 int64_t mta_conv_attn_decode_workspace(const mta_cache *cache, int64_t longest, int R, int S, int window);
 int mta_conv_attn_decode(const mta_cache *cache, const void *w, void *o, void *workspace, int64_t workspace_bytes, int64_t longest, int R, int S,
                          int window, float scale, int w_dtype, void *stream);
@@ -545,8 +545,8 @@ int mta_conv_attn_decode(const mta_cache *cache, const void *w, void *o, void *w
  * rows j = p - R2 + 1 .. p,  p_j = softmax( w_pre mix of conv_w(scale * raw) ),  o = ( w_post mix of conv_w2(p) at row p ) V;
  * what a row does not see counts as 0 ahead of either conv.  w is (heads, R, S), w2 (heads, R2, S2) or NULL with R2 = S2 = 1 (the
  * identity), w_pre and w_post (heads, heads) or NULL (the identity), all of dtype w_dtype; pre_group, post_group as group_size of
- * mta_headmix_fwd.  query_rows >= R + R2 - 1.  Everything else as mta_conv_attn_decode; the workspace (16-byte aligned) serves any
- * choice of NULL weights. */
+ * mta_headmix_fwd.  query_rows >= R + R2 - 1.  Everything else as mta_conv_attn_decode; the workspace serves any choice of
+ * NULL weights. */
 #define MTA_MAX_DECODE_KEYS (1 << 23) /* `longest` of mta_decode (a launch has 65535 blocks of some 200 keys) */
 int64_t mta_decode_workspace(const mta_cache *cache, int64_t longest, int R, int S, int R2, int S2, int pre_group, int post_group, int window);
 int mta_decode(const mta_cache *cache, const void *w, const void *w_pre, const void *w2, const void *w_post, void *o, void *workspace,

@@ -264,7 +264,7 @@ extern "C" int mta_conv_attn_decode(const mta_cache *c, const void *w, void *o, 
     if (const int e = check_args(c, longest, R, S, window)) return e;
     if (!w || !o) return MTA_ERR_NULL;
     if (dtype_size(w_dtype) == 0) return MTA_ERR_DTYPE;
-    if (!aligned_to(w, dtype_size(w_dtype)) || !aligned_to(o, dtype_size(c->dtype)) || !aligned_to(workspace, 8)) return MTA_ERR_ALIGN;
+    if (!aligned_to(w, dtype_size(w_dtype)) || !aligned_to(o, dtype_size(c->dtype)) || !aligned_to(workspace, 16)) return MTA_ERR_ALIGN;
     plan p;
     if (const int e = plan_of(c, longest, R, S, window, p)) return e;
     const int64_t need = mta_conv_attn_decode_workspace(c, longest, R, S, window);

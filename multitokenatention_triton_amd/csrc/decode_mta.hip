@@ -576,7 +576,7 @@ int plan_of(const mta_cache *c, int64_t longest, int R, int S, int R2, int S2, b
     p.s1 = 0;
     p.s2 = p.s1 + B * H * R2 * p.span;
     p.stats = p.s2 + (pre ? B * H * R2 * p.span : 0);
-    p.p1 = p.stats + 2 * B * H * R2 * p.chunks;
+    p.p1 = p.stats + (2 * B * H * R2 * p.chunks + 3) / 4 * 4;   // (parts begin on 16 bytes; the others are whole vectors as they are)
     p.part = p.p1 + (post_conv ? B * H * p.span : 0);
     p.total = p.part + (p.v.joined ? (int64_t)p.v.items * H * D : 0);
     return MTA_OK;

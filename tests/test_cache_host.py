@@ -254,6 +254,27 @@ def test_abi_argument_codes():
     assert lib.mta_decode_workspace(ctypes.byref(c), 64, 3, 3, 3, 3, 3, 0, 0) == -5 and lib.mta_decode_workspace(ctypes.byref(c), 64, 3, 3, 3, 3, 0, 0, 0) > 0
 
 
+def test_workspaces_hold_whole_vectors():
+    """Kernels read and write every part of a workspace 16 bytes at a time: it begins on 16 bytes, and so does each of its parts, whatever is odd.
+    (The parts behind the rows' statistics end the workspace and are whole vectors themselves: its size shows where they begin.)"""
+    lib = _lib.load()
+    p = 1 << 20
+
+    def made(slots, heads, keys):
+        return _lib.Cache(k=p, v=p, q=p, table=p, state=p, n_pages=4096, slots=slots, max_pages=-(-keys // 64), page=64, heads=heads, kv_heads=heads, head_dim=64,
+                          query_rows=32, dtype=0)
+
+    for slots, heads, r2, keys in ((3, 5, 7, 200), (3, 5, 7, 700), (1, 1, 3, 200), (1, 1, 1, 1), (3, 3, 9, 2817), (5, 7, 5, 769), (2, 4, 4, 300)):
+        c = made(slots, heads, keys)
+        assert lib.mta_decode_workspace(ctypes.byref(c), keys, 3, 3, r2, 3, 0, 0, 0) % 16 == 0, (slots, heads, r2, keys)
+    c = made(3, 5, 4096)
+    size = lib.mta_conv_attn_decode_workspace(ctypes.byref(c), 4096, 3, 3, 0)
+    assert size > 0
+    for off, code in ((4, -6), (8, -6)):
+        assert lib.mta_conv_attn_decode(ctypes.byref(c), p, p, p + off, size, 4096, 3, 3, 0, 0.1, 0, None) == code
+        assert lib.mta_decode(ctypes.byref(c), p, p, p, p, p, p + off, 1 << 40, 4096, 3, 3, 3, 3, 0, 0, 0, 0.1, 0, None) == code
+
+
 def test_longest_rows():
     """Multi-Token Attention's rows go as far as its launches do, and no size on the way wraps round; single-pass attention's go further."""
     lib = _lib.load()
