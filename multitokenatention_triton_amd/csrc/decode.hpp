@@ -48,9 +48,9 @@ __device__ __forceinline__ slot_step step_of(const decode_args &a, int b, int ol
 {
     const int had = a.state[b], got = a.state[a.slots + b];
     slot_step s = {0, 0, 0};
-    if (got <= 0) return s;
+    if (had < 0 || got < 0 || (got > 0 && had > a.longest - got)) { s.n = -1; return s; }   // (had + got may pass 32 bits)
+    if (got == 0) return s;
     s.n = had + got;
-    if (had < 0 || s.n <= 0 || s.n > a.longest) { s.n = -1; return s; }
     if (a.window > 0) {
         s.lo = s.n > a.window ? s.n - a.window : 0;
         s.base = s.lo > older ? (s.lo - older) & ~15 : 0;   // (the first key of the oldest output row)

@@ -560,6 +560,23 @@ def test_entries_that_are_no_pages():
     assert torch.equal(seq.cache.k.nan_to_num(7.0), pools[0].nan_to_num(7.0)) and torch.equal(seq.cache.v.nan_to_num(7.0), pools[1].nan_to_num(7.0))
 
 
+def test_states_that_are_none():
+    """Negative numbers and sums that pass 32 bits in a slot's state: NaN, also for slots that sit the step out; a long slot that sits it out is none of these."""
+    seq, conv, full, w, more = _pair(torch.bfloat16, [70] * 7)
+    for module in (conv, full):
+        seq.cache._upload(everything=True)
+        good = module.decode(seq.cache)
+        for slot, (had, got) in enumerate(((70, -3), (-1, 0), (-70, -1), (2 ** 31 - 5, 10), (69, 2 ** 31 - 1), (70, 0))):
+            seq.cache.state[0, slot], seq.cache.state[1, slot] = had, got
+        out = module.decode(seq.cache)
+        assert out[:5].isnan().all() and not out[5].any() and torch.equal(out[6], good[6])
+    pools = [x.clone().nan_to_num(7.0) for x in (seq.cache.k, seq.cache.v, seq.cache.q)]
+    seq.cache.state[1, 4], seq.cache.state[1, 6] = 0, 0
+    seq.cache.append(*[torch.ones(7, 4, 70, 64, dtype=torch.bfloat16, device="cuda")] * 3)   # (what has no page is dropped)
+    assert all(torch.equal(x.nan_to_num(7.0), y) for x, y in zip((seq.cache.k, seq.cache.v), pools))
+    assert all(torch.equal(seq.cache.q[b].nan_to_num(7.0), pools[2][b]) for b in (0, 1, 2, 4, 5, 6))
+
+
 def test_pools_beyond_32_bits():
     """Pages whose elements lie beyond 2**31, and bytes beyond 2**32."""
     h, d, page = 2, 128, 64
