@@ -256,6 +256,8 @@ class PagedCache:
         freed = sum(1 for p, times in going.items() if times == self._uses[p])
         if len(partial) * len(targets) > len(self._free) + freed:
             raise RuntimeError(f"the cache has {len(self._free) + freed} free pages, {len(partial) * len(targets)} are needed")
+        if partial and targets and not self.k.is_cuda:
+            raise RuntimeError(f"the cache lives on {self.k.device}: pages are copied on an AMD GPU only (there is no CPU path)")
         for slot in targets:
             self._release(slot)
         pairs = []

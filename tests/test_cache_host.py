@@ -140,6 +140,17 @@ def test_mark_appended():
     assert c.lengths == [0, 32, 0]
 
 
+def test_refused_fork_changes_nothing():
+    """Pages that cannot be copied are found out before anything is released."""
+    c = cache()
+    c.extend([20, 30, 0])
+    c.mark_appended()
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        c.fork(0, [1, 2])
+    consistent(c)
+    assert c.lengths == [20, 30, 0] and c.pages_of(0) == [0, 1] and c.pages_of(1) == [2, 3] and c.state.tolist() == [[0, 0, 0], [20, 30, 0]]
+
+
 def test_compact_without_moves():
     c = cache()
     assert c.compact() == 0
