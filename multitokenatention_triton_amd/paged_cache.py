@@ -151,7 +151,13 @@ class PagedCache:
         return slot
 
     def _capturing(self) -> bool:
-        return self.k.is_cuda and torch.cuda.is_current_stream_capturing()
+        """Whether the calls go into a graph: on the cache's device, where the work is queued, whatever the current one is."""
+        if not self.k.is_cuda:
+            return False
+        if torch.cuda.current_device() == self.k.device.index:   # (as nearly always, and a switch costs microseconds)
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self.k.device):
+            return torch.cuda.is_current_stream_capturing()
 
     def _eager(self, what: str) -> None:
         if self._capturing():
@@ -222,7 +228,7 @@ class PagedCache:
         if xk.dim() == 4 and xk.size(2) < max(self._added):
             raise ValueError(f"extend made room for up to {max(self._added)} tokens, append got {xk.size(2)}")
         _lib.host().cache_append(self.k, self.v, self.q, self.table, self.state, xq, xk, xv)
-        if not self._capturing():
+        if self._due and not self._capturing():
             self._due = False
 
     def mark_appended(self) -> None:

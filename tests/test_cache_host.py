@@ -151,6 +151,42 @@ def test_refused_fork_changes_nothing():
     assert c.lengths == [20, 30, 0] and c.pages_of(0) == [0, 1] and c.pages_of(1) == [2, 3] and c.state.tolist() == [[0, 0, 0], [20, 30, 0]]
 
 
+def test_capture_is_looked_for_on_the_device_of_the_cache(monkeypatch):
+    """Which stream is being captured is asked on the cache's own device, whatever the current one is."""
+    current, capturing = ["cuda:0"], "cuda:1"
+
+    class device:
+        def __init__(self, d):
+            self.d = str(d)
+
+        def __enter__(self):
+            current.append(self.d)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: int(current[-1][-1]))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[-1] == capturing)
+
+    class Pool:
+        is_cuda = True
+
+        def __init__(self, where, pool):
+            self.device, self.size = torch.device(where), pool.size
+
+    for where, longest in (("cuda:1", 80), ("cuda:0", 7), ("cuda:2", 7)):
+        c = cache()
+        c.extend([7, 0, 0])
+        c.k = Pool(where, c.k)
+        assert c.longest == longest
+        if longest == 80:
+            with pytest.raises(RuntimeError, match="between replays"):
+                c.compact()
+        else:
+            assert c.compact() == 1
+
+
 def test_compact_without_moves():
     c = cache()
     assert c.compact() == 0
