@@ -71,6 +71,7 @@ class TritonConvAttention(nn.Module):
 
     def decode(self, cache, softmax_scale=None, window=0):
         """The row of the newest token of every slot of a ``PagedCache`` that got tokens in its last ``extend``: (slots, H, 1, D),
-        zeros for the other slots.  Causal; ``window``: a row sees that many keys at most, itself included (0: all).  What
-        forward() rounds to the dtype between its stages stays in fp32 here.  No gradients."""
+        zeros for the other slots.  Causal, whatever ``self.causal`` says (forward() takes it as an argument and does not read
+        that either); ``window``: a row sees that many keys at most, itself included (0: all).  What forward() rounds to the dtype
+        between its stages stays in fp32 here.  No gradients."""
         return _lib.host().conv_attn_decode(cache.k, cache.v, cache.q, cache.table, cache.state, cache.longest, self.weight.detach(), softmax_scale, window)
