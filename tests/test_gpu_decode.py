@@ -293,6 +293,50 @@ def test_mta_weights_of_other_dtypes():
     check(module.decode(seq.cache)[0, 0], *seq.want(0, w, d ** -0.5, pre=pre.half(), w2=w2, post=post))
 
 
+# ---- the module's own forward() ---------------------------------------------------------------------------------------------
+def _close_to_forward(got, whole, bounds):
+    """decode() is within `bounds` of the formulas, forward() in fp32 within what its own tests hold it to, rtol 1e-4 and atol 1e-5: so far apart they
+    may be.  (A tap, a row or a head out of place is some hundredths.)"""
+    got, whole = got.double().cpu(), whole.double().cpu()
+    off = (got - whole).abs() - (bounds + 2 ** -24 * got.abs() + 1e-4 * whole.abs() + 1e-5)
+    assert off.max() <= 0, f"{float((got - whole).abs().max())} apart, {float(off.max())} too far"
+
+
+@pytest.mark.parametrize("r,s", [(3, 3), (6, 11), (3, 4), (2, 6), (1, 2)])
+@pytest.mark.parametrize("n", [1, 5, 77, 300])
+def test_conv_attention_is_the_last_row_of_forward(r, s, n):
+    h, d, dtype = 4, 64, torch.float32
+    seq = Sequences([n, n], h, h, d, dtype, 16, r, scatter=False)
+    w = conv_weight(h, r, s, dtype, seq.gen)
+    module = conv_module(w)
+    with torch.no_grad():
+        whole, _ = module(*(x[:, :, :n].contiguous().cuda() for x in (seq.q, seq.k, seq.v)), True, 0.2)
+    got = module.decode(seq.cache, 0.2)
+    _close_to_forward(got[:, :, 0], whole[:, :, -1], torch.stack([seq.want(b, w, 0.2)[1] for b in range(2)]))
+
+
+@pytest.mark.parametrize("h,r,s,r2,s2,group,window", [(8, 3, 3, 3, 3, 0, 0), (8, 6, 11, 0, 0, 4, 0), (4, 5, 7, 2, 4, 2, 0), (4, 2, 4, 4, 6, 0, 0), (16, 3, 5, 5, 3, 0, 0),
+                                                      (8, 6, 11, 0, 0, 2, 40), (4, 3, 4, 3, 5, 0, 100)])
+@pytest.mark.parametrize("n", [1, 5, 77, 304])
+def test_mta_is_the_last_row_of_forward(h, r, s, r2, s2, group, window, n):
+    d, dtype = 64, torch.float32
+    seq = Sequences([n, n], h, h, d, dtype, 16, r + max(r2, 3) - 1, scatter=False)
+    w, w2 = conv_weight(h, r, s, dtype, seq.gen), conv_weight(h, r2, s2, dtype, seq.gen) if r2 else None
+    pre, post = head_weight(h, group or h, dtype, seq.gen), head_weight(h, group or h, dtype, seq.gen)
+    declared = dict(pre_head_group=group, post_head_group=group, post_conv_identity=not r2) if group else {}
+    module = mta_module(w, pre, w2, post, **declared)
+    mask = None
+    if window:
+        at = torch.arange(n, device="cuda")
+        mask = ((at[None] <= at[:, None]) & (at[None] > at[:, None] - window)).expand(2, 1, n, n)
+        module.use_mask = True
+    with torch.no_grad():
+        whole = module(*(x[:, :, :n].contiguous().cuda() for x in (seq.q, seq.k, seq.v)), mask, None)
+    got = module.decode(seq.cache, window=window)
+    bounds = torch.stack([seq.want(b, w, d ** -0.5, pre=pre, w2=w2, post=post, window=window)[1] for b in range(2)])
+    _close_to_forward(got[:, 0], whole[:, -1], bounds)
+
+
 # ---- a serving loop ------------------------------------------------------------------------------------------------------------
 def test_prompt_then_tokens_then_fork_then_compact():
     """Prompts, a few steps, a beam that splits, one that ends, pages moved together, more steps: every step against whole sequences."""
