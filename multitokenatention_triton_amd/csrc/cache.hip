@@ -66,8 +66,8 @@ struct copy_args {
 static_assert(sizeof(copy_args) <= 4096, "arguments of a launch");
 
 // A workgroup moves 8 KB of one page of one pool.  The pairs travel as arguments: no copy to the device, nothing to wait for.  1000 pages of 2 x 128 KB,
-// us: two vectors per lane 96, four 105, eight 158 (as for reading, more in flight is slower); non-temporal stores 82, 480 pairs a launch one launch's work in
-// place of four 64.
+// us, at 240 pairs a launch: two vectors per lane 96, four 105, eight 158 (as for reading, more in flight is slower); non-temporal stores 82.  480 pairs a
+// launch, three launches in place of five: 88 with ordinary stores, 74 with non-temporal ones.
 template <bool STREAM> __global__ __launch_bounds__(256) void cache_copy_pages_kernel(const copy_args a)
 {
     const int2 pair = a.pair[blockIdx.y];

@@ -119,7 +119,7 @@ __device__ __forceinline__ int wave_scan(int v)
 // How the slots' keys are shared out over workgroups.  The host knows the longest slot at most (a captured graph: not even that), so the
 // device does it: every slot's keys in steps, `per` of them to an item.  Items of one size, however different the lengths, and all that live
 // next to each other in the grid, which deals its workgroups over the XCDs in turn: with a grid of (split, head, slot) short slots left
-// whole XCDs idle (conv-attention, 16 slots of 1k to 8k keys 204 us, now 153; MTA, 16 slots of 512 to 4k keys 142, now 84).
+// whole XCDs idle (conv-attention, 16 slots of 1k to 8k keys 204 us that way, 153 this way; MTA, 16 slots of 512 to 4k keys 142, 84).
 // per: `target` items are one round of workgroups that are all resident (an item costs some 5 us beside its keys - the table, queries, weights,
 // the first loads, the results - which a second round pays again: 8k keys of 32 heads 30 us in one round, 37 in two); where they come
 // out long, four times as many, which even out the end (16 slots of up to 8k keys 165 us in items of 25 steps, 153 in 7).

@@ -140,7 +140,8 @@ class PagedCache:
 
     @property
     def longest(self) -> int:
-        """What sizes a decode: the longest slot; while a graph is captured, what the table has room for."""
+        """What sizes a decode: the longest slot; while a graph is captured, what the table has room for (``max_pages`` pages, which also
+        size the workspace of ``MTAAttentionTriton.decode``; beyond 2**23 positions that is refused)."""
         if self._capturing():
             return self.table.size(1) * self.page_size
         return max(1, max(self._lengths))
