@@ -512,8 +512,8 @@ int mta_probe_conv_kernel(const void *w, int64_t C, int R, int S, int w_dtype, i
  * extension; a slot that got none sits the step out.  Query head h reads key head h / (heads / kv_heads).  table and state are
  * read on the device when the work runs: a captured graph follows them.
  *
- * Kernels check what they read there.  A slot whose state is no state of this cache (new ones and more tokens than `longest` of the call
- * or than its row of the table has room for, a negative number), or one of whose pages is none of 0 .. n_pages - 1, gets NaN for
+ * Kernels check what they read there.  A slot whose state is no state of this cache (a negative number; new tokens that make it longer than
+ * `longest` of the call or than its row of the table has room for), or one of whose pages is none of 0 .. n_pages - 1, gets NaN for
  * a result, and nothing is read or written through such an entry. */
 typedef struct mta_cache {
     void *k, *v, *q;
